@@ -457,6 +457,99 @@ tatara_status tatara_gdn_decode_batch_indirect(tatara_ctx* ctx, void* stream, co
 tatara_status tatara_lanes_advance(tatara_ctx* ctx, void* stream, tatara_attn_lane* attn_lanes_device,
                                    uint32_t n_attn, tatara_gdn_lane* gdn_lanes_device, uint32_t n_gdn);
 
+/* ---- paged KV cache ----------------------------------------------------------------------
+ * A cache whose slots live in pages of two pools, for lanes that grow and shrink independently: slot s
+ * of lane i is row s % page_slots of page page_table[i][s / page_slots].  It has no counterpart in the
+ * reference, whose lanes own contiguous stripes.  Slots are filled in order; which token a slot holds
+ * stops being a matter of order once tatara_paged_evict has moved rows, so a lane carries its slot count
+ * and its newest position apart, and `positions` tells the token of every slot.
+ *
+ * Everything about a token is read from device memory (the lane table, the page table), nothing but
+ * bounds is a kernel argument: calls may be captured in a CUDA graph and replayed, with
+ * tatara_paged_lanes_step as the node between tokens.  What the host cannot check is checked on the device
+ * before it is used: a lane with more than `max_keys` slots is left out (its output and its cache stay
+ * as they are), a page number >= n_pages is neither read nor written (its slots count as absent); either
+ * latches TATARA_CONTEXT_OUT_OF_RANGE for the next tatara_ctx_sync.  Lanes with keys == 0 are idle.
+ * Calls on different streams may run at the same time as long as they share no scratch and none writes
+ * what another touches.  Calls switch to the context's device and back. */
+typedef enum tatara_dtype { TATARA_BF16 = 0, TATARA_F16 = 1 } tatara_dtype;
+#define TATARA_MAX_GROUP 16u /* query heads per kv head of the paged decode */
+
+typedef struct tatara_paged_lane {
+    uint32_t keys;     /* slots in use, the newest token's included; 0 = idle lane                 */
+    uint32_t position; /* position of the newest token (>= keys - 1, larger once slots were evicted) */
+} tatara_paged_lane;
+
+/* Host-side description of one layer's cache; read during the call only. */
+typedef struct tatara_paged_cache {
+    void* keys;   /* element (page, kv head, row, dim) at page*page_stride + head*head_stride + row*slot_stride + dim */
+    void* values; /* same layout */
+    uint64_t page_stride, head_stride, slot_stride; /* elements, multiples of 8 */
+    const uint32_t* page_table; /* device, [table_lanes][table_pages]; entries of pages not yet in use are not read */
+    float* mass;                /* device, [table_lanes][kv_heads][table_pages*page_slots], or NULL: accumulated attention weight */
+    uint32_t* positions;        /* device, same shape, or NULL: position of the token in the slot  */
+    uint32_t table_lanes, table_pages;
+    uint32_t n_pages;           /* pages of each pool                                  */
+    uint32_t page_slots;        /* a multiple of 16, at most 1024                      */
+    uint32_t kv_heads, head_dim;/* head_dim 64, 128 or 256                             */
+    uint32_t dtype;             /* tatara_dtype of both pools, of the queries and of the outputs */
+    uint32_t reserved;
+} tatara_paged_cache;
+
+/* Appends rows: lane i's newest row_starts[i+1] - row_starts[i] slots (those before slot lanes[i].keys) get rows
+ * row_starts[i] .. of `keys` / `values`, element (row, kv head, dim) at row*row_stride + head*source_head_stride + dim
+ * (so a contiguous lane cache [kv head][capacity][dim] is a source as it is).  row_starts: device,
+ * [n_lanes + 1], ascending from 0; rows from row_starts[n_lanes] up to n_rows (padding) are not read.
+ * row_starts == NULL: row i belongs to lane i (n_rows == n_lanes).  The slots' mass is set to 0 and their
+ * positions to the tokens'.  A row whose slot would lie before slot 0 or beyond the page table is left out and
+ * latches TATARA_CONTEXT_OUT_OF_RANGE. */
+tatara_status tatara_paged_append(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
+                                  const tatara_paged_lane* lanes_device, uint32_t n_lanes, const void* keys,
+                                  const void* values, uint64_t row_stride, uint64_t source_head_stride,
+                                  const uint32_t* row_starts, uint32_t n_rows);
+
+/* tatara_attn_qk_rope_batch over pages: projection row i [9216] belongs to lane i; q / gate rows as there, K and V
+ * to slot keys - 1 at the lane's position.  bf16, 2 kv heads of 256.  The angle is reduced in double and each
+ * result rounded once, so rows agree with tatara_attn_qk_rope_batch (which rounds the normalised row to
+ * bf16 first) within that operator's roundings.  Idle lanes' q and gate rows stay as they are. */
+tatara_status tatara_attn_qk_rope_paged(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
+                                        const tatara_paged_lane* lanes_device, uint32_t n_lanes,
+                                        const void* projection, const void* q_weight, const void* k_weight,
+                                        void* q_out, void* gate_out, uint64_t projection_stride,
+                                        uint64_t query_stride);
+
+/* Decode attention of one new token per lane over its slots 0..keys-1, split over the length and joined.
+ * q, gate (or NULL: no gate), out: lane i's heads at i*query_stride + head*head_dim; q_heads a multiple of kv_heads,
+ * at most TATARA_MAX_GROUP per kv head; softmax(scale * q.k) v, times sigmoid(gate).  With cache->mass every slot's
+ * weight, summed over the query heads of its kv head, is added to its mass.  An idle lane's out row becomes
+ * zero.  max_keys: no lane holds more slots (it bounds the scratch; the
+ * page table's capacity serves when nothing better is known).  A lane's bits do not depend on the batch. */
+uint64_t tatara_attn_decode_paged_scratch_bytes(const tatara_paged_cache* cache, uint32_t n_lanes, uint32_t max_keys,
+                                                uint32_t q_heads);
+tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
+                                       const tatara_paged_lane* lanes_device, uint32_t n_lanes, uint32_t max_keys,
+                                       const void* q, const void* gate, uint32_t q_heads, uint64_t query_stride,
+                                       float scale, void* out, void* scratch, uint64_t scratch_bytes);
+
+/* Trims every lane with more than `keep` slots to `keep`, per kv head.  Slots are ranked: guarded ones first (the
+ * lane's first `sink` slots, and tokens among the `recent` newest positions), then by mass, largest first
+ * (not-a-number last); equals by the lower slot.  The first `keep` stay: those below slot `keep` where they are, the others
+ * move, in ascending order, into the slots below `keep` that were given up, in ascending order -- K and V rows,
+ * mass and position.  So no row moves that need not.  Slots from `keep` on are left as they are; tatara_paged_lanes_step
+ * then cuts the lane.  Needs mass, and positions where recent > 0; sink + recent <= keep.  Pages that two lanes share may
+ * hold only their first `sink` slots (nothing there is ever overwritten). */
+uint64_t tatara_paged_evict_scratch_bytes(const tatara_paged_cache* cache, uint32_t n_lanes, uint32_t max_keys,
+                                          uint32_t keep);
+tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
+                                 const tatara_paged_lane* lanes_device, uint32_t n_lanes, uint32_t max_keys,
+                                 uint32_t keep, uint32_t sink, uint32_t recent, void* scratch,
+                                 uint64_t scratch_bytes);
+
+/* Between tokens: every lane that is not idle is cut to `keep` slots (after the evictions of all layers that share the
+ * table; UINT32_MAX: no cut) and then moves on by `advance` tokens (keys and position). */
+tatara_status tatara_paged_lanes_step(tatara_ctx* ctx, void* stream, tatara_paged_lane* lanes_device, uint32_t n_lanes,
+                                      uint32_t keep, uint32_t advance);
+
 #ifdef __cplusplus
 }
 #endif

@@ -19,6 +19,7 @@ ATTN_PROJ = 9216
 GDN_PROJ, GDN_CONV, GDN_QK, GDN_V, GDN_HEADS, GDN_DIM = 12352, 8192, 4096, 4096, 32, 128
 RECORD_FLOATS = 258
 MAX_LANES = 256
+MAX_CONTEXT = 262144
 
 STATUS_NAMES = ["None", "InvalidBuffer", "ContextOutOfRange", "StateSlotMismatch",
                 "InvalidStreamGroup", "InvalidDispatchExtent", "InvalidDevice", "ScratchTooSmall",
@@ -49,6 +50,23 @@ class GdnLane(ctypes.Structure):
                 ("rec_in", ctypes.c_uint64), ("rec_out", ctypes.c_uint64)]
 
 
+class PagedCache(ctypes.Structure):
+    """tatara_paged_cache; made by :func:`paged_cache`, which also keeps the tensors alive."""
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p),
+                ("page_stride", ctypes.c_uint64), ("head_stride", ctypes.c_uint64), ("slot_stride", ctypes.c_uint64),
+                ("page_table", ctypes.c_void_p), ("mass", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("table_lanes", ctypes.c_uint32), ("table_pages", ctypes.c_uint32), ("n_pages", ctypes.c_uint32),
+                ("page_slots", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("head_dim", ctypes.c_uint32),
+                ("dtype", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
+
+    @property
+    def capacity(self) -> int:
+        """Slots that a lane's row of the page table can address."""
+        return self.table_pages * self.page_slots
+
+
+NO_CUT = 0xFFFFFFFF   # paged_lanes_step: keep every slot
+
 _lib = None
 
 
@@ -72,6 +90,14 @@ def lib() -> ctypes.CDLL:
         _lib.tatara_attn_partitions.restype = ctypes.c_uint32
         _lib.tatara_split_buffer_bytes.restype = ctypes.c_uint64
         _lib.tatara_ctx_get_policy.restype = ctypes.c_uint64
+        p, u32, u64 = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64
+        _lib.tatara_attn_decode_paged_scratch_bytes.restype = u64
+        _lib.tatara_paged_evict_scratch_bytes.restype = u64
+        _lib.tatara_paged_append.argtypes = [p, p, p, p, u32, p, p, u64, u64, p, u32]
+        _lib.tatara_attn_qk_rope_paged.argtypes = [p, p, p, p, u32, p, p, p, p, p, u64, u64]
+        _lib.tatara_attn_decode_paged.argtypes = [p, p, p, p, u32, u32, p, p, u32, u64, ctypes.c_float, p, p, u64]
+        _lib.tatara_paged_evict.argtypes = [p, p, p, p, u32, u32, u32, u32, u32, p, u64]
+        _lib.tatara_paged_lanes_step.argtypes = [p, p, p, u32, u32, u32]
     return _lib
 
 
@@ -111,6 +137,44 @@ def _ptr(t):
 
 _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
+
+
+def _address(t):
+    """A tensor's address as a plain integer, None for None: what a call with declared argument types takes as it is."""
+    return None if t is None else t.data_ptr()
+
+
+def paged_cache(keys, values, page_table, mass=None, positions=None) -> PagedCache:
+    """Describes a paged KV cache: pools [page][kv head][slot][dim] (views of any layout whose dim is contiguous, both
+    pools alike), page table [lane][page] int32, mass / positions [lane][kv head][page * slots] f32 / int32 or None."""
+    import torch
+    kinds = {torch.bfloat16: 0, torch.float16: 1}
+    if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or keys.dtype != values.dtype or keys.dtype not in kinds:
+        raise ValueError("paged_cache: keys and values are alike, [page][kv head][slot][dim] in bf16 or f16")
+    if keys.stride(3) != 1:
+        raise ValueError("paged_cache: the dims of a row are contiguous")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise ValueError("paged_cache: page_table is [lane][page] int32, contiguous")
+    pages, heads, slots, dim = keys.shape
+    plane = (page_table.shape[0], heads, page_table.shape[1] * slots)
+    for name, t, dtype in (("mass", mass, torch.float32), ("positions", positions, torch.int32)):
+        if t is not None and (tuple(t.shape) != plane or t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"paged_cache: {name} is {list(plane)} {dtype}, contiguous")
+    if any(t is not None and t.device != keys.device for t in (values, page_table, mass, positions)):
+        raise ValueError("paged_cache: tensors on one device")
+    c = PagedCache(keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2),
+                   page_table.data_ptr(), _address(mass), _address(positions), page_table.shape[0], page_table.shape[1],
+                   pages, slots, heads, dim, kinds[keys.dtype], 0)
+    c.tensors = (keys, values, page_table, mass, positions)
+    return c
+
+
+def decode_paged_scratch_bytes(cache: PagedCache, n_lanes: int, max_keys: int, q_heads: int) -> int:
+    return int(lib().tatara_attn_decode_paged_scratch_bytes(ctypes.byref(cache), _u32(n_lanes), _u32(max_keys), _u32(q_heads)))
+
+
+def paged_evict_scratch_bytes(cache: PagedCache, n_lanes: int, max_keys: int, keep: int) -> int:
+    return int(lib().tatara_paged_evict_scratch_bytes(ctypes.byref(cache), _u32(n_lanes), _u32(max_keys), _u32(keep)))
 
 
 class Context:
@@ -341,6 +405,79 @@ class Context:
     def lanes_advance(self, attn_lanes_device, n_attn, gdn_lanes_device, n_gdn, stream=None):
         self._check(lib().tatara_lanes_advance(self._h, self._stream(stream), _ptr(attn_lanes_device), _u32(n_attn),
                                                _ptr(gdn_lanes_device), _u32(n_gdn)))
+
+    # ---- paged KV cache.  lanes: int32 CUDA tensor [lane][2] = slots in use, newest position
+    @staticmethod
+    def _paged_rows(what, t, cache, n, row):
+        """n rows of `row` elements each in the cache's type, one stride apart; returns that stride."""
+        shape, strides = t.shape, t.stride()
+        inner = 1
+        for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
+            if size != 1 and stride != inner:
+                inner = -1
+                break
+            inner *= size
+        if inner != row or shape[0] < n or t.dtype != cache.tensors[0].dtype:
+            raise ValueError(f"{what}: at least {n} rows of {row} contiguous elements in the cache's type")
+        return strides[0] if shape[0] > 1 else row
+
+    @staticmethod
+    def _paged_lanes(lanes):
+        import torch
+        if lanes.dim() != 2 or lanes.shape[1] != 2 or lanes.dtype != torch.int32 or not lanes.is_contiguous():
+            raise ValueError("lanes: [lane][2] int32, contiguous")
+        return lanes.data_ptr(), lanes.shape[0]
+
+    def paged_append(self, cache, lanes, keys, values, row_starts=None, stream=None):
+        """keys, values: [row][kv head][dim] views with one layout; row_starts: int32 [lanes + 1], or None for one row per lane."""
+        import torch
+        at, n = self._paged_lanes(lanes)
+        if keys.dim() != 3 or keys.shape != values.shape or keys.stride() != values.stride() or keys.stride(2) != 1 or \
+                keys.dtype != cache.tensors[0].dtype or values.dtype != keys.dtype or tuple(keys.shape[1:]) != (cache.kv_heads, cache.head_dim):
+            raise ValueError("paged_append: keys and values are alike, [row][kv head][dim] in the cache's type")
+        if row_starts is not None and (row_starts.dtype != torch.int32 or row_starts.numel() != n + 1 or not row_starts.is_contiguous()):
+            raise ValueError("paged_append: row_starts is int32 [lanes + 1]")
+        head_stride = keys.stride(1) if cache.kv_heads > 1 else cache.head_dim
+        row_stride = keys.stride(0) if keys.shape[0] > 1 else cache.kv_heads * cache.head_dim
+        self._check(lib().tatara_paged_append(self._h, self._stream(stream), ctypes.byref(cache), at, n, keys.data_ptr(), values.data_ptr(),
+                                              row_stride, head_stride, _address(row_starts), keys.shape[0]))
+
+    def attn_qk_rope_paged(self, cache, lanes, projection, q_weight, k_weight, q_out, gate_out, stream=None):
+        """projection [lane][9216]; q_out, gate_out [lane][16][256], rows of any one stride."""
+        at, n = self._paged_lanes(lanes)
+        stride = self._paged_rows("attn_qk_rope_paged: q_out", q_out, cache, n, Q_HEADS * HEAD_DIM)
+        if self._paged_rows("attn_qk_rope_paged: gate_out", gate_out, cache, n, Q_HEADS * HEAD_DIM) != stride:
+            raise ValueError("attn_qk_rope_paged: q_out and gate_out have one stride")
+        self._check(lib().tatara_attn_qk_rope_paged(
+            self._h, self._stream(stream), ctypes.byref(cache), at, n, projection.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+            q_out.data_ptr(), gate_out.data_ptr(), self._paged_rows("attn_qk_rope_paged: projection", projection, cache, n, ATTN_PROJ), stride))
+
+    def attn_decode_paged(self, cache, lanes, q, gate, out, scratch, max_keys=None, scale=None, stream=None):
+        """q, gate (or None), out: [lane][q head][dim], rows of any one stride.  Adds to the cache's mass where it has one.
+        scale: head_dim ** -0.5 unless given; max_keys: the page table's capacity unless given."""
+        at, n = self._paged_lanes(lanes)
+        if q.dim() != 3:
+            raise ValueError("attn_decode_paged: q is [lane][q head][dim]")
+        q_heads, dim = q.shape[1], cache.head_dim
+        stride = self._paged_rows("attn_decode_paged: q", q, cache, n, q_heads * dim)
+        for name, t in (("gate", gate), ("out", out)):
+            if t is not None and self._paged_rows("attn_decode_paged: " + name, t, cache, n, q_heads * dim) != stride:
+                raise ValueError("attn_decode_paged: q, gate and out have one stride")
+        self._check(lib().tatara_attn_decode_paged(
+            self._h, self._stream(stream), ctypes.byref(cache), at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
+            q.data_ptr(), _address(gate), q_heads, stride, dim ** -0.5 if scale is None else scale, out.data_ptr(), scratch.data_ptr(),
+            scratch.numel() * scratch.element_size()))
+
+    def paged_evict(self, cache, lanes, keep, scratch, sink=0, recent=0, max_keys=None, stream=None):
+        """Trims every lane to at most `keep` slots; paged_lanes_step(lanes, keep=keep) then cuts the lane table."""
+        at, n = self._paged_lanes(lanes)
+        self._check(lib().tatara_paged_evict(
+            self._h, self._stream(stream), ctypes.byref(cache), at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
+            keep, sink, recent, scratch.data_ptr(), scratch.numel() * scratch.element_size()))
+
+    def paged_lanes_step(self, lanes, keep=NO_CUT, advance=1, stream=None):
+        at, n = self._paged_lanes(lanes)
+        self._check(lib().tatara_paged_lanes_step(self._h, self._stream(stream), at, n, keep, advance))
 
     # ---- speculative-decode support: GDN tape and replay
     def gdn_prepare_tape(self, projection, conv_in, conv_weights, qk, value, z, conv_out, rows, conv_tape, tape_layer,

@@ -15,7 +15,7 @@
 // (tb::partition_keys), every record is computed by one warp-order-fixed procedure and the
 // combine walks records in index order, so a lane's output bits do not depend on which other
 // lanes share the launch or on which CTA ran which item.
-#include "common.cuh"
+#include "warp_tiles.cuh"
 
 #include <cstring>
 #include <mutex>
@@ -68,44 +68,6 @@ struct DecParams {
     DecLane lane[N];
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-// K / V rows are read once per token: they are marked evict-first in L2 so that the stream does
-// not push out what the step re-reads (q, gate, the partial records).
-__device__ __forceinline__ uint64_t l2_evict_first_policy() {
-    uint64_t policy;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-    return policy;
-}
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t src_bytes, uint64_t policy) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;\n" ::"r"(dst), "l"(src),
-                 "r"(src_bytes), "l"(policy)
-                 : "memory");
-}
-// Asks for `bytes` (a multiple of 16, from a 16-byte aligned address) to be brought into L2; nothing
-// is written to shared memory or registers, so the request may precede the dependency wait even for
-// rows the predecessor is still writing (L2 is the point of coherence: a later store updates the line).
-__device__ __forceinline__ void l2_prefetch_bulk(const void* src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(kPending) : "memory");
-}
-__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                            uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t& r0, uint32_t& r1,
-                                                  uint32_t& r2, uint32_t& r3) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-                 : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-                 : "r"(addr));
-}
 // D(16x8) = A(16x16) * B(16x8) + C with rows 8..15 of A zero: only rows 0..7 are kept.
 __device__ __forceinline__ void mma_top_rows(float& d0, float& d1, uint32_t a0, uint32_t a2,
                                              uint32_t b0, uint32_t b1) {
@@ -123,12 +85,6 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// Transposes an 8x8 matrix of 16-bit elements held one row per four lanes (lane 4g + t: row g, columns 2t, 2t+1).
-__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
-    uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
-    return d;
 }
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);

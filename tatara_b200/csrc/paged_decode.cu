@@ -1,0 +1,621 @@
+// Decode attention of one new token per lane over a paged KV cache, split over the cache's length and joined.
+//
+//   out[h] = sum_s p[h][s] v[s],  p[h][s] = softmax over s < keys of scale q[h].k[s]
+//
+// One pass over K and V with a running maximum and sum.  A lane's slots are cut into partitions; a work item
+// (lane, kv head, partition) leaves, for every query head of the group, the un-normalised sum of its values, the
+// maximum m of its scores (times log2 e) and the sum l of 2^(s - m).  The join weighs the partitions with 2^(m - M),
+// divides and applies the gate; where the cache carries a mass it adds 2^(s - M) / L of every slot, summed over the
+// group, to it -- the scores were put aside in f32 by the first kernel, 4 bytes a head beside the 4 x head_dim of K and V.
+//
+// Bound: HBM.  A slot of a kv head is 4 x head_dim bytes and 4 x head_dim x group flops, 8 flops a byte for a group of 8, two orders
+// below the tensor cores' balance, so mma.sync fragments out of shared memory carry the products and everything is
+// arranged around the stream of K and V rows: every warp owns a ring of cp.async slices (16 slots of K and V) that runs ahead
+// across items, and a slice never leaves its page, so one page-table entry (held by a lane, 32 slices at a time) serves it.
+//
+// The partition of a lane depends on its own slot count and the cache's geometry alone, each record is made in a fixed order and the join
+// walks the records in order: a lane's bits are the same alone and in any batch.
+#include "paged.cuh"
+
+#include <cmath>
+
+namespace tb {
+
+constexpr uint32_t kPdWarps = 4, kPdThreads = kPdWarps * 32, kPdStages = 3;
+constexpr float kPdLog2e = 1.4426950408889634f;
+constexpr uint32_t kPdMinPart = 128;          // slots of the shortest partition: two slices for each warp
+constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinDims = 64;
+constexpr uint32_t kJoinPhases = 8;           // the join adds partitions f, f + 8, ... in phase f, then the phases in order
+
+// CTAs of the first kernel that share an SM: the rings of 256 / head_dim of them fill its shared memory.
+__host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim) { return 256u / head_dim; }
+// The cut of a lane of n slots: one item for every resident CTA once the lane is long enough, at least 128 slots each.
+__host__ __device__ inline uint32_t pd_per_wave(uint32_t kv_heads, uint32_t head_dim) {
+    const uint32_t p = kSmCount * pd_ctas(head_dim) / kv_heads;
+    return p == 0u ? 1u : p;
+}
+__host__ __device__ inline uint32_t pd_part_slots(uint32_t n, uint32_t per_wave) {
+    if (n <= per_wave * kPdMinPart) return kPdMinPart;
+    return ((n + per_wave - 1u) / per_wave + kPagedSlice - 1u) / kPagedSlice * kPagedSlice;
+}
+__host__ __device__ inline uint32_t pd_parts(uint32_t n, uint32_t per_wave) {
+    const uint32_t p = pd_part_slots(n, per_wave);
+    return (n + p - 1u) / p;
+}
+
+struct PagedDecodeParams {
+    PagedView cache;
+    const tatara_paged_lane* lanes;
+    const uint8_t* q;
+    const uint8_t* gate;
+    uint8_t* out;
+    float* sums;       // [lane][q head][part][head_dim]
+    float2* stats;     // [lane][q head][part]: maximum (log2 units), sum
+    float* scores;     // [lane][kv head][max_keys rounded up to 16][group rounded up to 8], log2 units; null without a mass
+    uint64_t query_stride;
+    uint32_t n_lanes, max_keys, q_heads, group, per_wave;
+    uint32_t parts;        // parts of the longest lane: the stride of sums and stats
+    uint32_t score_slots;  // max_keys rounded up to 16
+    float scale_log2e;
+};
+
+template <typename T> struct Half;
+template <> struct Half<__nv_bfloat16> {
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ float load(const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); }
+    static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v); }
+};
+template <> struct Half<__half> {
+    static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ float load(const uint8_t* p) { return __half2float(*reinterpret_cast<const __half*>(p)); }
+    static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__half*>(p) = __float2half_rn(v); }
+};
+
+// The items of every lane, counted by each CTA for itself: item_start[i] (n_lanes + 1 entries) and the lanes' slot
+// counts, 0 for a lane that is idle or refused.  Called by all threads.
+template <uint32_t kThreads>
+__device__ __forceinline__ void scan_items(const PagedDecodeParams& p, uint32_t* item_start, uint32_t* lane_keys, uint32_t* warp_total, bool latch) {
+    constexpr uint32_t kOwn = (TATARA_MAX_LANES + kThreads - 1u) / kThreads, kWarps = kThreads / 32u;
+    const uint32_t first = threadIdx.x * kOwn, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    uint32_t mine = 0, count[kOwn];
+#pragma unroll
+    for (uint32_t j = 0; j < kOwn; ++j) {
+        const uint32_t i = first + j;
+        uint32_t n = 0;
+        if (i < p.n_lanes) {
+            n = __ldcg(&p.lanes[i].keys);
+            if (n > p.max_keys) {
+                if (latch) latch_out_of_range(p.cache, i);
+                n = 0;
+            }
+            lane_keys[i] = n;
+        }
+        count[j] = n == 0u ? 0u : pd_parts(n, p.per_wave) * p.cache.kv_heads;
+        mine += count[j];
+    }
+    uint32_t incl = mine;
+#pragma unroll
+    for (uint32_t off = 1; off < 32; off <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
+        if (lane >= off) incl += v;
+    }
+    if (lane == 31u) warp_total[warp] = incl;
+    __syncthreads();
+    uint32_t at = incl - mine;
+#pragma unroll
+    for (uint32_t w = 0; w < kWarps; ++w)
+        if (w < warp) at += warp_total[w];
+#pragma unroll
+    for (uint32_t j = 0; j < kOwn; ++j) {
+        if (first + j <= p.n_lanes) item_start[first + j] = at;
+        at += count[j];
+    }
+    if (threadIdx.x == kThreads - 1u && kOwn * kThreads == p.n_lanes) item_start[p.n_lanes] = at;
+    __syncthreads();
+}
+
+struct PagedItem {
+    uint32_t lane, kv, part, begin, slots;   // slots of the partition, from slot `begin` of the lane
+};
+__device__ __forceinline__ PagedItem item_at(const PagedDecodeParams& p, const uint32_t* item_start, const uint32_t* lane_keys, uint32_t item) {
+    uint32_t lo = 0, hi = p.n_lanes;   // last lane with item_start <= item (lanes without items share their successor's)
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (item_start[mid] <= item) lo = mid; else hi = mid;
+    }
+    const uint32_t local = item - item_start[lo], n = lane_keys[lo], size = pd_part_slots(n, p.per_wave);
+    PagedItem it;
+    it.lane = lo;
+    it.part = local / p.cache.kv_heads;
+    it.kv = local - it.part * p.cache.kv_heads;
+    it.begin = it.part * size;
+    it.slots = min(size, n - it.begin);
+    return it;
+}
+
+template <int D>
+struct PdGeometry {
+    static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kSlice = kPagedSlice * kRow, kStage = 2 * kSlice;
+    static constexpr uint32_t kRing = kPdStages * kStage;                 // a warp's
+    static constexpr uint32_t kMergeRow = D + 4;                          // floats: the padding spreads the heads over the banks
+    static_assert(8 * kMergeRow * 4 <= kStage, "a warp's eight rows of the merge lie in one ring stage");
+    static constexpr uint32_t kSmem = kPdWarps * kRing + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 8) * 4;
+};
+
+// kTiles: tiles of eight query heads, 1 or 2.
+template <typename T, int D, int kTiles>
+__global__ void __launch_bounds__(kPdThreads, pd_ctas(D))
+paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
+    using G = PdGeometry<D>;
+    constexpr uint32_t kSteps = D / 16;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
+    float2* merge_ml = reinterpret_cast<float2*>(smem + kPdWarps * G::kRing);
+    uint32_t* item_start = reinterpret_cast<uint32_t*>(merge_ml + kPdWarps * 8);
+    uint32_t* lane_keys = item_start + TATARA_MAX_LANES + 1;
+    uint32_t* warp_total = lane_keys + TATARA_MAX_LANES;
+    const uint32_t ring = smem_u32(smem + warp * G::kRing);
+    const uint64_t policy = l2_evict_first_policy();
+    wait_for_predecessor();
+    release_dependents();
+    scan_items<kPdThreads>(p, item_start, lane_keys, warp_total, blockIdx.x == 0);
+    const uint32_t total = item_start[p.n_lanes];
+
+    // ---- the warp's stream of slices, kPdStages - 1 ahead of the arithmetic, across items
+    uint32_t next_item = blockIdx.x, turn = 0, issued = 0, consumed = 0;
+    uint32_t pages = 0;            // lane j: page of the warp's slice 32 * (turn / 32) + j of the item
+    uint32_t absent = 0;           // bit s: the page of ring stage s does not exist
+    PagedItem pi{};
+    bool more = next_item < total;
+    if (more) pi = item_at(p, item_start, lane_keys, next_item);
+    auto issue = [&]() {
+        // the next slice of this warp: of the current item, or of the next item that has one for it
+        while (more && (warp + turn * kPdWarps) * kPagedSlice >= pi.slots) {
+            next_item += gridDim.x;
+            turn = 0;
+            more = next_item < total;
+            if (more) pi = item_at(p, item_start, lane_keys, next_item);
+        }
+        if (more) {
+            if ((turn & 31u) == 0u) {
+                const uint32_t slot = (warp + (turn + lane) * kPdWarps) * kPagedSlice;
+                if (slot < pi.slots) pages = __ldcg(p.cache.page_table + uint64_t(pi.lane) * p.cache.table_pages + (pi.begin + slot) / p.cache.page_slots);
+            }
+            const uint32_t page = __shfl_sync(0xffffffffu, pages, turn & 31u);
+            const uint32_t first = (warp + turn * kPdWarps) * kPagedSlice;
+            const bool exists = page < p.cache.n_pages;
+            const uint32_t rows = exists ? min(kPagedSlice, pi.slots - first) : 0u;
+            const uint32_t stage = issued % kPdStages;
+            absent = (absent & ~(1u << stage)) | (exists ? 0u : 1u << stage);
+            if (!exists && lane == 0) latch_out_of_range(p.cache, pi.lane);
+            const uint64_t offset = exists ? page * p.cache.page_bytes + pi.kv * p.cache.head_bytes +
+                                                 ((pi.begin + first) % p.cache.page_slots) * p.cache.slot_bytes
+                                           : 0ull;
+            const uint32_t chunk = lane % G::kChunks, row0 = lane / G::kChunks;
+            const uint8_t* ksrc = p.cache.keys + offset + chunk * 16u;
+            const uint8_t* vsrc = p.cache.values + offset + chunk * 16u;
+            const uint32_t dst0 = ring + stage * G::kStage;
+#pragma unroll
+            for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
+                const uint32_t row = r + row0;
+                const bool live = row < rows;    // rows behind the partition and absent pages read nothing: zeros
+                const uint64_t off = live ? row * p.cache.slot_bytes : 0ull;
+                const uint32_t dst = dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4);
+                cp_async_16(dst, ksrc + off, live ? 16u : 0u, policy);
+                cp_async_16(dst + G::kSlice, vsrc + off, live ? 16u : 0u, policy);
+            }
+            ++turn;
+        }
+        cp_async_commit();
+        ++issued;
+    };
+#pragma unroll
+    for (uint32_t i = 0; i + 1 < kPdStages; ++i) issue();
+
+    // Products run transposed, so that the 16 rows of the A operand are slots (scores) and dims (values) and the heads sit
+    // in the eight columns: S^T = K Q^T, O^T += V^T P^T.  A by ldmatrix out of the XOR-swizzled slice, Q and P^T in registers.
+    const uint32_t lm_j = lane >> 3, lm_r = lane & 7u;
+    const uint32_t k_row = ((lm_j & 1u) * 8u + lm_r) * G::kRow, k_chunk = lm_j >> 1;
+    const uint32_t v_row = ((lm_j >> 1) * 8u + lm_r) * G::kRow, v_chunk = lm_j & 1u;
+
+    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
+        const PagedItem ci = item_at(p, item_start, lane_keys, item);
+        uint32_t qf[kTiles][kSteps][2];
+#pragma unroll
+        for (uint32_t nt = 0; nt < kTiles; ++nt) {
+            const uint32_t head = nt * 8u + g;
+            const uint32_t* row = reinterpret_cast<const uint32_t*>(
+                p.q + (ci.lane * p.query_stride + uint64_t(ci.kv * p.group + (head < p.group ? head : 0u)) * D) * 2u);
+#pragma unroll
+            for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                qf[nt][ks][0] = head < p.group ? __ldcg(row + ks * 8u + t) : 0u;
+                qf[nt][ks][1] = head < p.group ? __ldcg(row + ks * 8u + 4u + t) : 0u;
+            }
+        }
+        float o[kTiles][kSteps][4], m[kTiles][2], l[kTiles][2];
+#pragma unroll
+        for (uint32_t nt = 0; nt < kTiles; ++nt) {
+#pragma unroll
+            for (uint32_t ks = 0; ks < kSteps; ++ks) o[nt][ks][0] = o[nt][ks][1] = o[nt][ks][2] = o[nt][ks][3] = 0.0f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
+        float* score_base = p.scores == nullptr ? nullptr
+                            : p.scores + ((uint64_t(ci.lane) * p.cache.kv_heads + ci.kv) * p.score_slots + ci.begin) * (kTiles * 8u);
+
+        for (uint32_t slice = warp; slice * kPagedSlice < ci.slots; slice += kPdWarps) {
+            issue();
+            cp_async_wait<kPdStages - 1>();
+            __syncwarp();
+            const uint32_t stage = consumed % kPdStages;
+            const uint32_t kst = ring + stage * G::kStage, vst = kst + G::kSlice;
+            const bool exists = ((absent >> stage) & 1u) == 0u;
+            float s[kTiles][4], s2[kTiles][4];
+#pragma unroll
+            for (uint32_t nt = 0; nt < kTiles; ++nt)
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.0f;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kSteps; ks += 2) {
+                uint32_t a0, a1, a2, a3;
+                ldmatrix_x4(kst + k_row + (((ks * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+#pragma unroll
+                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1]);
+                ldmatrix_x4(kst + k_row + ((((ks + 1u) * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+#pragma unroll
+                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s2[nt], a0, a1, a2, a3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+            }
+            // lane (g, t): slots g and g + 8 of the slice, heads 2t and 2t + 1 of each tile
+            const uint32_t slot0 = slice * kPagedSlice + g;
+            const bool live0 = exists && slot0 < ci.slots, live1 = exists && slot0 + 8u < ci.slots;
+            float alpha[kTiles][2];
+            uint32_t pb[kTiles][2];
+            bool rescale = false;
+#pragma unroll
+            for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                float x[4];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) x[i] = (i < 2 ? live0 : live1) ? (s[nt][i] + s2[nt][i]) * p.scale_log2e : -INFINITY;
+                if (score_base != nullptr) {
+                    float* at = score_base + uint64_t(slot0) * (kTiles * 8u) + nt * 8u + 2u * t;
+                    if (slot0 < ci.slots) *reinterpret_cast<float2*>(at) = make_float2(x[0], x[1]);
+                    if (slot0 + 8u < ci.slots) *reinterpret_cast<float2*>(at + 8u * kTiles * 8u) = make_float2(x[2], x[3]);
+                }
+                float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+#pragma unroll
+                for (uint32_t off = 4; off < 32; off <<= 1) {
+                    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+                    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+                }
+                const float n0 = fmaxf(m[nt][0], mx0), n1 = fmaxf(m[nt][1], mx1);
+                // nothing seen yet (an absent page, scores of -inf): every weight is 2^(-inf) = 0 against any finite base
+                const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
+                alpha[nt][0] = exp2f(m[nt][0] - b0);
+                alpha[nt][1] = exp2f(m[nt][1] - b1);
+                const float p0 = exp2f(x[0] - b0), p1 = exp2f(x[1] - b1), p2 = exp2f(x[2] - b0), p3 = exp2f(x[3] - b1);
+                l[nt][0] = l[nt][0] * alpha[nt][0] + (p0 + p2);
+                l[nt][1] = l[nt][1] * alpha[nt][1] + (p1 + p3);
+                m[nt][0] = n0;
+                m[nt][1] = n1;
+                // the weights are rounded to the cache's type for the second product: half a step each, of random sign
+                pb[nt][0] = movmatrix_trans(Half<T>::pack(p0, p1));   // slots 2t, 2t+1 of head g
+                pb[nt][1] = movmatrix_trans(Half<T>::pack(p2, p3));   // slots 2t+8, 2t+9 of head g
+                rescale = rescale || alpha[nt][0] != 1.0f || alpha[nt][1] != 1.0f;
+            }
+            // a factor of exactly 1 leaves every bit as it is, so the rescale is skipped when no lane needs it
+            rescale = __any_sync(0xffffffffu, rescale);
+#pragma unroll
+            for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                uint32_t a0, a1, a2, a3;
+                ldmatrix_x4_trans(vst + v_row + (((ks * 2u + v_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+#pragma unroll
+                for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                    if (rescale) {
+                        o[nt][ks][0] *= alpha[nt][0];
+                        o[nt][ks][1] *= alpha[nt][1];
+                        o[nt][ks][2] *= alpha[nt][0];
+                        o[nt][ks][3] *= alpha[nt][1];
+                    }
+                    Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                }
+            }
+            __syncwarp();   // every lane is done with this stage before it is refilled
+            ++consumed;
+        }
+
+        // ---- the four warps' parts of the item, joined eight heads at a time.  Each warp lays its rows over the ring stage
+        // that it read last: kPdStages - 1 stages are in flight or waiting, so that one is free until the next issue().
+        const uint32_t free_stage = (consumed + kPdStages - 1u) % kPdStages;
+        float* merge_mine = reinterpret_cast<float*>(smem + warp * G::kRing + free_stage * G::kStage);
+        if (lane == 0) warp_total[warp] = free_stage;
+#pragma unroll
+        for (uint32_t nt = 0; nt < kTiles; ++nt) {
+#pragma unroll
+            for (uint32_t off = 4; off < 32; off <<= 1) {
+                l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], off);
+                l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], off);
+            }
+            float* mo = merge_mine + 2u * t * G::kMergeRow + g;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                mo[ks * 16u] = o[nt][ks][0];
+                mo[G::kMergeRow + ks * 16u] = o[nt][ks][1];
+                mo[ks * 16u + 8u] = o[nt][ks][2];
+                mo[G::kMergeRow + ks * 16u + 8u] = o[nt][ks][3];
+            }
+            if (g == 0) {
+                merge_ml[warp * 8u + 2u * t] = make_float2(m[nt][0], l[nt][0]);
+                merge_ml[warp * 8u + 2u * t + 1u] = make_float2(m[nt][1], l[nt][1]);
+            }
+            __syncthreads();
+            const uint32_t h = threadIdx.x >> 4, head = nt * 8u + h;
+            if (head < p.group) {
+                float wt[kPdWarps], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kPdWarps; ++w) top = fmaxf(top, merge_ml[w * 8u + h].x);
+#pragma unroll
+                for (uint32_t w = 0; w < kPdWarps; ++w) {
+                    const float2 ml = merge_ml[w * 8u + h];
+                    wt[w] = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+                    sum = fmaf(wt[w], ml.y, sum);
+                }
+                const uint64_t record = (uint64_t(ci.lane) * p.q_heads + ci.kv * p.group + head) * p.parts + ci.part;
+                float4* dst = reinterpret_cast<float4*>(p.sums + record * D);
+#pragma unroll
+                for (uint32_t d4 = threadIdx.x & 15u; d4 < D / 4; d4 += 16u) {
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (uint32_t w = 0; w < kPdWarps; ++w) {
+                        const float4 v = *reinterpret_cast<const float4*>(smem + w * G::kRing + warp_total[w] * G::kStage +
+                                                                          (h * G::kMergeRow + d4 * 4u) * 4u);
+                        acc.x = fmaf(wt[w], v.x, acc.x);
+                        acc.y = fmaf(wt[w], v.y, acc.y);
+                        acc.z = fmaf(wt[w], v.z, acc.z);
+                        acc.w = fmaf(wt[w], v.w, acc.w);
+                    }
+                    dst[d4] = acc;
+                }
+                if ((threadIdx.x & 15u) == 0u) p.stats[record] = make_float2(top, sum);
+            }
+            __syncthreads();
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// ---- the join -----------------------------------------------------------------------------
+// CTAs 0 .. lanes*q_heads*D/64 - 1 finish 64 dims of a head each; the others walk the items again and add the weights to the mass.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads)
+paged_join_kernel(const __grid_constant__ PagedDecodeParams p) {
+    __shared__ uint32_t item_start[TATARA_MAX_LANES + 1], lane_keys[TATARA_MAX_LANES], warp_total[kJoinWarps];
+    __shared__ float weight[kSmCount * 4];                 // at most per_wave partitions
+    __shared__ float red[kJoinWarps];
+    __shared__ __align__(16) float acc_s[kJoinPhases][kJoinDims];
+    __shared__ float2 final_ml[16];
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    constexpr uint32_t kSlices = D / kJoinDims;
+    const uint32_t pieces = p.n_lanes * p.q_heads * kSlices;
+    wait_for_predecessor();
+    release_dependents();
+    if (blockIdx.x < pieces) {
+        const uint32_t slice = blockIdx.x % kSlices, rest = blockIdx.x / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
+        const uint32_t n = __ldcg(&p.lanes[row].keys);
+        if (n > p.max_keys) return;                        // refused: its row stays as it is
+        const uint32_t parts = n == 0u ? 0u : pd_parts(n, p.per_wave);
+        const uint64_t record = (uint64_t(row) * p.q_heads + head) * p.parts;
+        const uint32_t pair = threadIdx.x & 31u, phase = threadIdx.x >> 5;
+        const uint64_t at = (row * p.query_stride + uint64_t(head) * D + slice * kJoinDims + threadIdx.x) * 2u;
+        float gate = 0.0f;
+        if (threadIdx.x < kJoinDims && p.gate != nullptr) gate = Half<T>::load(p.gate + at);
+        // the first partitions' sums are asked for before their weights are known
+        constexpr uint32_t kAhead = 10;
+        float2 v[kAhead];
+        const float* base = p.sums + record * D + slice * kJoinDims + pair * 2u;
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t part = phase + i * kJoinPhases;
+            v[i] = part < parts ? __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D)) : make_float2(0.0f, 0.0f);
+        }
+        float top = -INFINITY;
+        for (uint32_t part = threadIdx.x; part < parts; part += kJoinThreads) top = fmaxf(top, __ldcg(&p.stats[record + part]).x);
+#pragma unroll
+        for (uint32_t off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (lane == 0) red[warp] = top;
+        __syncthreads();
+        top = red[0];
+#pragma unroll
+        for (uint32_t w = 1; w < kJoinWarps; ++w) top = fmaxf(top, red[w]);
+        __syncthreads();
+        float sum = 0.0f;
+        for (uint32_t part = threadIdx.x; part < parts; part += kJoinThreads) {
+            const float2 ml = __ldcg(&p.stats[record + part]);
+            const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+            weight[part] = w;
+            sum = fmaf(w, ml.y, sum);
+        }
+#pragma unroll
+        for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == 0) red[warp] = sum;
+        __syncthreads();
+        float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+        for (uint32_t i = 0; i < kAhead; ++i) {
+            const uint32_t part = phase + i * kJoinPhases;
+            if (part < parts) {
+                a0 = fmaf(weight[part], v[i].x, a0);
+                a1 = fmaf(weight[part], v[i].y, a1);
+            }
+        }
+        for (uint32_t part = phase + kAhead * kJoinPhases; part < parts; part += kJoinPhases) {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D));
+            a0 = fmaf(weight[part], x.x, a0);
+            a1 = fmaf(weight[part], x.y, a1);
+        }
+        *reinterpret_cast<float2*>(&acc_s[phase][pair * 2u]) = make_float2(a0, a1);
+        __syncthreads();
+        if (threadIdx.x < kJoinDims) {
+            float num = 0.0f, den = 0.0f;
+#pragma unroll
+            for (uint32_t ph = 0; ph < kJoinPhases; ++ph) num += acc_s[ph][threadIdx.x];
+#pragma unroll
+            for (uint32_t w = 0; w < kJoinWarps; ++w) den += red[w];
+            float r = den == 0.0f ? 0.0f : num / den;      // no slot at all: zero
+            if (p.gate != nullptr) r *= 1.0f / (1.0f + expf(-gate));
+            Half<T>::store(p.out + at, r);
+        }
+        return;
+    }
+    scan_items<kJoinThreads>(p, item_start, lane_keys, warp_total, false);
+    const uint32_t total = item_start[p.n_lanes], row_floats = (p.group + 7u) / 8u * 8u;
+    for (uint32_t item = blockIdx.x - pieces; item < total; item += gridDim.x - pieces) {
+        const PagedItem it = item_at(p, item_start, lane_keys, item);
+        const uint32_t parts = pd_parts(lane_keys[it.lane], p.per_wave);
+        for (uint32_t h = warp; h < p.group; h += kJoinWarps) {
+            const float2* st = p.stats + (uint64_t(it.lane) * p.q_heads + it.kv * p.group + h) * p.parts;
+            float top = -INFINITY, sum = 0.0f;
+            for (uint32_t part = lane; part < parts; part += 32u) top = fmaxf(top, __ldcg(&st[part]).x);
+#pragma unroll
+            for (uint32_t off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            for (uint32_t part = lane; part < parts; part += 32u) {
+                const float2 ml = __ldcg(&st[part]);
+                sum = fmaf(ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top), ml.y, sum);
+            }
+#pragma unroll
+            for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            if (lane == 0) final_ml[h] = make_float2(top == -INFINITY ? 0.0f : top, sum == 0.0f ? 0.0f : 1.0f / sum);
+        }
+        __syncthreads();
+        const uint64_t head_row = uint64_t(it.lane) * p.cache.kv_heads + it.kv;
+        const float* scores = p.scores + (head_row * p.score_slots + it.begin) * row_floats;
+        float* mass = p.cache.mass + head_row * p.cache.capacity + it.begin;
+        for (uint32_t slot = threadIdx.x; slot < it.slots; slot += kJoinThreads) {
+            const float* x = scores + uint64_t(slot) * row_floats;
+            float w = 0.0f;
+            for (uint32_t h0 = 0; h0 < p.group; h0 += 4u) {
+                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + h0));
+                const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    if (h0 + j < p.group) w = fmaf(exp2f(e[j] - final_ml[h0 + j].x), final_ml[h0 + j].y, w);
+            }
+            mass[slot] += w;
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------
+struct PagedDecodeLayout {
+    uint32_t per_wave, parts, score_slots, row_floats;
+    uint64_t stats_at, scores_at, bytes;
+};
+static PagedDecodeLayout pd_layout(const tatara_paged_cache& c, uint32_t n_lanes, uint32_t max_keys, uint32_t q_heads) {
+    PagedDecodeLayout l{};
+    l.per_wave = pd_per_wave(c.kv_heads, c.head_dim);
+    const uint32_t shortest = (max_keys + kPdMinPart - 1u) / kPdMinPart;   // pd_parts(n) <= both for every n <= max_keys
+    l.parts = shortest < l.per_wave ? shortest : l.per_wave;
+    l.score_slots = (max_keys + kPagedSlice - 1u) / kPagedSlice * kPagedSlice;
+    l.row_floats = (q_heads / c.kv_heads + 7u) / 8u * 8u;
+    const uint64_t records = uint64_t(n_lanes) * q_heads * l.parts;
+    l.stats_at = records * c.head_dim * 4u;
+    l.scores_at = (l.stats_at + records * 8u + 255u) / 256u * 256u;
+    l.bytes = l.scores_at + (c.mass == nullptr ? 0u : uint64_t(n_lanes) * c.kv_heads * l.score_slots * l.row_floats * 4u);
+    return l;
+}
+
+template <typename T, int D, int kTiles>
+static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, const PagedDecodeParams& p) {
+    static bool configured[64] = {false};
+    if (!configured[ctx->device & 63]) {
+        if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 PdGeometry<D>::kSmem) != cudaSuccess)
+            return check_launch(ctx, "attn_decode_paged: shared memory attribute");
+        configured[ctx->device & 63] = true;
+    }
+    const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, resident = uint64_t(ctx->sm_count) * pd_ctas(D);
+    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < resident ? items : resident)), kPdThreads,
+                        PdGeometry<D>::kSmem, stream, p);
+    const tatara_status st = check_launch(ctx, "attn_decode_paged");
+    if (st != TATARA_OK) return st;
+    const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
+    const uint64_t walkers = p.cache.mass == nullptr ? 0u : items < 4u * ctx->sm_count ? items : 4u * ctx->sm_count;
+    (void)launch_staged(paged_join_kernel<T, D>, dim3(pieces + uint32_t(walkers)), kJoinThreads, 0u, stream, p);
+    return check_launch(ctx, "attn_decode_paged: join");
+}
+
+template <typename T>
+static tatara_status pick_paged_decode(tatara_ctx* ctx, cudaStream_t stream, const PagedDecodeParams& p, uint32_t head_dim) {
+    const bool wide = p.group > 8u;
+    switch (head_dim) {
+    case 64: return wide ? launch_paged_decode<T, 64, 2>(ctx, stream, p) : launch_paged_decode<T, 64, 1>(ctx, stream, p);
+    case 128: return wide ? launch_paged_decode<T, 128, 2>(ctx, stream, p) : launch_paged_decode<T, 128, 1>(ctx, stream, p);
+    default: return wide ? launch_paged_decode<T, 256, 2>(ctx, stream, p) : launch_paged_decode<T, 256, 1>(ctx, stream, p);
+    }
+}
+
+} // namespace tb
+
+using namespace tb;
+
+extern "C" uint64_t tatara_attn_decode_paged_scratch_bytes(const tatara_paged_cache* cache, uint32_t n_lanes, uint32_t max_keys,
+                                                           uint32_t q_heads) {
+    if (cache == nullptr || cache->kv_heads == 0 || cache->head_dim == 0 || cache->head_dim > 256u || max_keys > TATARA_MAX_CONTEXT) return 0;
+    return pd_layout(*cache, n_lanes, max_keys, q_heads).bytes;
+}
+
+extern "C" tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
+                                                  const tatara_paged_lane* lanes_device, uint32_t n_lanes, uint32_t max_keys,
+                                                  const void* q, const void* gate, uint32_t q_heads, uint64_t query_stride,
+                                                  float scale, void* out, void* scratch, uint64_t scratch_bytes) {
+    if (ctx == nullptr) return TATARA_INVALID_BUFFER;
+    const tatara_status st = check_paged(ctx, cache, lanes_device, n_lanes);
+    if (st != TATARA_OK) return st;
+    if (!q || !out || !scratch) return fail(ctx, TATARA_INVALID_BUFFER, "attn_decode_paged: null buffer");
+    if (!aligned(q, 4) || !aligned(gate, 2) || !aligned(out, 2) || !aligned(scratch, 16))
+        return fail(ctx, TATARA_INVALID_BUFFER, "attn_decode_paged: misaligned buffer");
+    if (q_heads == 0 || q_heads % cache->kv_heads != 0 || q_heads / cache->kv_heads > TATARA_MAX_GROUP)
+        return fail(ctx, TATARA_INVALID_DISPATCH_EXTENT, "attn_decode_paged: query heads per kv head");
+    if (query_stride < uint64_t(q_heads) * cache->head_dim || query_stride % 2u)
+        return fail(ctx, TATARA_INVALID_DISPATCH_EXTENT, "attn_decode_paged: query stride");
+    if (!std::isfinite(scale)) return fail(ctx, TATARA_INVALID_DISPATCH_EXTENT, "attn_decode_paged: scale");
+    if (max_keys == 0 || max_keys > cache->table_pages * cache->page_slots || max_keys > TATARA_MAX_CONTEXT)
+        return fail(ctx, TATARA_CONTEXT_OUT_OF_RANGE, "attn_decode_paged: max_keys beyond the page table or the longest context");
+    const PagedDecodeLayout l = pd_layout(*cache, n_lanes, max_keys, q_heads);
+    if (scratch_bytes < l.bytes) return fail(ctx, TATARA_SCRATCH_TOO_SMALL, "attn_decode_paged: scratch");
+    PagedDecodeParams p{};
+    p.cache = paged_view(ctx, *cache);
+    p.lanes = lanes_device;
+    p.q = static_cast<const uint8_t*>(q);
+    p.gate = static_cast<const uint8_t*>(gate);
+    p.out = static_cast<uint8_t*>(out);
+    p.sums = static_cast<float*>(scratch);
+    p.stats = reinterpret_cast<float2*>(static_cast<uint8_t*>(scratch) + l.stats_at);
+    p.scores = cache->mass == nullptr ? nullptr : reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + l.scores_at);
+    p.query_stride = query_stride;
+    p.n_lanes = n_lanes;
+    p.max_keys = max_keys;
+    p.q_heads = q_heads;
+    p.group = q_heads / cache->kv_heads;
+    p.per_wave = l.per_wave;
+    p.parts = l.parts;
+    p.score_slots = l.score_slots;
+    p.scale_log2e = scale * kPdLog2e;
+    const DeviceGuard guard(ctx);
+    return cache->dtype == TATARA_BF16 ? pick_paged_decode<__nv_bfloat16>(ctx, static_cast<cudaStream_t>(stream), p, cache->head_dim)
+                                       : pick_paged_decode<__half>(ctx, static_cast<cudaStream_t>(stream), p, cache->head_dim);
+}
