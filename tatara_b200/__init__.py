@@ -139,15 +139,25 @@ _u32 = ctypes.c_uint32
 _u64 = ctypes.c_uint64
 
 
-def _address(t):
-    """A tensor's address as a plain integer, None for None: what a call with declared argument types takes as it is."""
-    return None if t is None else t.data_ptr()
+_torch = None
+_current_stream = None
+
+
+def _bind_torch():
+    """torch owns the memory and the streams of a paged cache; it is imported with the first one."""
+    global _torch, _current_stream
+    if _torch is None:
+        import torch
+        # the handle alone: torch.cuda.current_stream makes a Stream object for every call, 2 us beside a 5 us launch
+        _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
+        _torch = torch
+    return _torch
 
 
 def paged_cache(keys, values, page_table, mass=None, positions=None) -> PagedCache:
     """Describes a paged KV cache: pools [page][kv head][slot][dim] (views of any layout whose dim is contiguous, both
     pools alike), page table [lane][page] int32, mass / positions [lane][kv head][page * slots] f32 / int32 or None."""
-    import torch
+    torch = _bind_torch()
     kinds = {torch.bfloat16: 0, torch.float16: 1}
     if keys.dim() != 4 or keys.shape != values.shape or keys.stride() != values.stride() or keys.dtype != values.dtype or keys.dtype not in kinds:
         raise ValueError("paged_cache: keys and values are alike, [page][kv head][slot][dim] in bf16 or f16")
@@ -163,9 +173,11 @@ def paged_cache(keys, values, page_table, mass=None, positions=None) -> PagedCac
     if any(t is not None and t.device != keys.device for t in (values, page_table, mass, positions)):
         raise ValueError("paged_cache: tensors on one device")
     c = PagedCache(keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2),
-                   page_table.data_ptr(), _address(mass), _address(positions), page_table.shape[0], page_table.shape[1],
-                   pages, slots, heads, dim, kinds[keys.dtype], 0)
+                   page_table.data_ptr(), None if mass is None else mass.data_ptr(), None if positions is None else positions.data_ptr(),
+                   page_table.shape[0], page_table.shape[1], pages, slots, heads, dim, kinds[keys.dtype], 0)
     c.tensors = (keys, values, page_table, mass, positions)
+    c.torch_dtype, c.device = keys.dtype, keys.get_device()
+    c.ref = ctypes.addressof(c)
     return c
 
 
@@ -407,77 +419,82 @@ class Context:
                                                _ptr(gdn_lanes_device), _u32(n_gdn)))
 
     # ---- paged KV cache.  lanes: int32 CUDA tensor [lane][2] = slots in use, newest position
+    def _paged_stream(self, stream):
+        """The stream's handle; None: the current stream of the context's device (whichever device is current)."""
+        if stream is None:
+            return _current_stream(self.device)
+        return stream if isinstance(stream, int) else stream.cuda_stream
+
     @staticmethod
     def _paged_rows(what, t, cache, n, row):
         """n rows of `row` elements each in the cache's type, one stride apart; returns that stride."""
-        shape, strides = t.shape, t.stride()
-        inner = 1
-        for size, stride in zip(reversed(shape[1:]), reversed(strides[1:])):
-            if size != 1 and stride != inner:
-                inner = -1
-                break
-            inner *= size
-        if inner != row or shape[0] < n or t.dtype != cache.tensors[0].dtype:
-            raise ValueError(f"{what}: at least {n} rows of {row} contiguous elements in the cache's type")
-        return strides[0] if shape[0] > 1 else row
+        shape = t.shape
+        if shape[0] >= n and t.dtype is cache.torch_dtype and t.get_device() == cache.device:
+            if t.is_contiguous():
+                if t.numel() == shape[0] * row:
+                    return row
+            elif t[0].numel() == row and t[0].is_contiguous():
+                return t.stride(0)
+        raise ValueError(f"{what}: at least {n} rows of {row} contiguous elements in the cache's type, on its device")
 
-    @staticmethod
-    def _paged_lanes(lanes):
-        import torch
-        if lanes.dim() != 2 or lanes.shape[1] != 2 or lanes.dtype != torch.int32 or not lanes.is_contiguous():
-            raise ValueError("lanes: [lane][2] int32, contiguous")
-        return lanes.data_ptr(), lanes.shape[0]
+    def _paged_lanes(self, lanes, cache=None):
+        _bind_torch()
+        shape = lanes.shape
+        if len(shape) != 2 or shape[1] != 2 or lanes.dtype is not _torch.int32 or not lanes.is_contiguous() or \
+                lanes.get_device() != self.device or cache is not None and cache.device != self.device:
+            raise ValueError("lanes: [lane][2] int32, contiguous, on the context's device as the cache is")
+        return lanes.data_ptr(), shape[0]
 
     def paged_append(self, cache, lanes, keys, values, row_starts=None, stream=None):
         """keys, values: [row][kv head][dim] views with one layout; row_starts: int32 [lanes + 1], or None for one row per lane."""
-        import torch
-        at, n = self._paged_lanes(lanes)
-        if keys.dim() != 3 or keys.shape != values.shape or keys.stride() != values.stride() or keys.stride(2) != 1 or \
-                keys.dtype != cache.tensors[0].dtype or values.dtype != keys.dtype or tuple(keys.shape[1:]) != (cache.kv_heads, cache.head_dim):
+        at, n = self._paged_lanes(lanes, cache)
+        shape, strides = keys.shape, keys.stride()
+        if len(shape) != 3 or shape[1] != cache.kv_heads or shape[2] != cache.head_dim or strides[2] != 1 or values.shape != shape or \
+                values.stride() != strides or keys.dtype is not cache.torch_dtype or values.dtype is not cache.torch_dtype or keys.get_device() != cache.device or \
+                values.get_device() != cache.device:
             raise ValueError("paged_append: keys and values are alike, [row][kv head][dim] in the cache's type")
-        if row_starts is not None and (row_starts.dtype != torch.int32 or row_starts.numel() != n + 1 or not row_starts.is_contiguous()):
+        if row_starts is not None and (row_starts.dtype is not _torch.int32 or row_starts.numel() != n + 1 or not row_starts.is_contiguous()):
             raise ValueError("paged_append: row_starts is int32 [lanes + 1]")
-        head_stride = keys.stride(1) if cache.kv_heads > 1 else cache.head_dim
-        row_stride = keys.stride(0) if keys.shape[0] > 1 else cache.kv_heads * cache.head_dim
-        self._check(lib().tatara_paged_append(self._h, self._stream(stream), ctypes.byref(cache), at, n, keys.data_ptr(), values.data_ptr(),
-                                              row_stride, head_stride, _address(row_starts), keys.shape[0]))
+        # (a dimension of one has no stride that means anything)
+        self._check(lib().tatara_paged_append(
+            self._h, self._paged_stream(stream), cache.ref, at, n, keys.data_ptr(), values.data_ptr(),
+            strides[0] if shape[0] > 1 else shape[1] * shape[2], strides[1] if shape[1] > 1 else shape[2],
+            None if row_starts is None else row_starts.data_ptr(), shape[0]))
 
     def attn_qk_rope_paged(self, cache, lanes, projection, q_weight, k_weight, q_out, gate_out, stream=None):
         """projection [lane][9216]; q_out, gate_out [lane][16][256], rows of any one stride."""
-        at, n = self._paged_lanes(lanes)
+        at, n = self._paged_lanes(lanes, cache)
         stride = self._paged_rows("attn_qk_rope_paged: q_out", q_out, cache, n, Q_HEADS * HEAD_DIM)
         if self._paged_rows("attn_qk_rope_paged: gate_out", gate_out, cache, n, Q_HEADS * HEAD_DIM) != stride:
             raise ValueError("attn_qk_rope_paged: q_out and gate_out have one stride")
         self._check(lib().tatara_attn_qk_rope_paged(
-            self._h, self._stream(stream), ctypes.byref(cache), at, n, projection.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
+            self._h, self._paged_stream(stream), cache.ref, at, n, projection.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
             q_out.data_ptr(), gate_out.data_ptr(), self._paged_rows("attn_qk_rope_paged: projection", projection, cache, n, ATTN_PROJ), stride))
 
     def attn_decode_paged(self, cache, lanes, q, gate, out, scratch, max_keys=None, scale=None, stream=None):
         """q, gate (or None), out: [lane][q head][dim], rows of any one stride.  Adds to the cache's mass where it has one.
         scale: head_dim ** -0.5 unless given; max_keys: the page table's capacity unless given."""
-        at, n = self._paged_lanes(lanes)
-        if q.dim() != 3:
-            raise ValueError("attn_decode_paged: q is [lane][q head][dim]")
+        at, n = self._paged_lanes(lanes, cache)
         q_heads, dim = q.shape[1], cache.head_dim
         stride = self._paged_rows("attn_decode_paged: q", q, cache, n, q_heads * dim)
-        for name, t in (("gate", gate), ("out", out)):
-            if t is not None and self._paged_rows("attn_decode_paged: " + name, t, cache, n, q_heads * dim) != stride:
-                raise ValueError("attn_decode_paged: q, gate and out have one stride")
+        if self._paged_rows("attn_decode_paged: out", out, cache, n, q_heads * dim) != stride or \
+                gate is not None and self._paged_rows("attn_decode_paged: gate", gate, cache, n, q_heads * dim) != stride:
+            raise ValueError("attn_decode_paged: q, gate and out have one stride")
         self._check(lib().tatara_attn_decode_paged(
-            self._h, self._stream(stream), ctypes.byref(cache), at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
-            q.data_ptr(), _address(gate), q_heads, stride, dim ** -0.5 if scale is None else scale, out.data_ptr(), scratch.data_ptr(),
-            scratch.numel() * scratch.element_size()))
+            self._h, self._paged_stream(stream), cache.ref, at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
+            q.data_ptr(), None if gate is None else gate.data_ptr(), q_heads, stride, dim ** -0.5 if scale is None else scale,
+            out.data_ptr(), scratch.data_ptr(), scratch.numel() * scratch.element_size()))
 
     def paged_evict(self, cache, lanes, keep, scratch, sink=0, recent=0, max_keys=None, stream=None):
         """Trims every lane to at most `keep` slots; paged_lanes_step(lanes, keep=keep) then cuts the lane table."""
-        at, n = self._paged_lanes(lanes)
+        at, n = self._paged_lanes(lanes, cache)
         self._check(lib().tatara_paged_evict(
-            self._h, self._stream(stream), ctypes.byref(cache), at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
+            self._h, self._paged_stream(stream), cache.ref, at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
             keep, sink, recent, scratch.data_ptr(), scratch.numel() * scratch.element_size()))
 
     def paged_lanes_step(self, lanes, keep=NO_CUT, advance=1, stream=None):
         at, n = self._paged_lanes(lanes)
-        self._check(lib().tatara_paged_lanes_step(self._h, self._stream(stream), at, n, keep, advance))
+        self._check(lib().tatara_paged_lanes_step(self._h, self._paged_stream(stream), at, n, keep, advance))
 
     # ---- speculative-decode support: GDN tape and replay
     def gdn_prepare_tape(self, projection, conv_in, conv_weights, qk, value, z, conv_out, rows, conv_tape, tape_layer,

@@ -21,17 +21,19 @@
 
 namespace tb {
 
-constexpr uint32_t kPdWarps = 4, kPdThreads = kPdWarps * 32, kPdStages = 3;
+constexpr uint32_t kPdWarps = 4, kPdThreads = kPdWarps * 32;
 constexpr float kPdLog2e = 1.4426950408889634f;
 constexpr uint32_t kPdMinPart = 128;          // slots of the shortest partition: two slices for each warp
 constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinDims = 64;
 constexpr uint32_t kJoinPhases = 8;           // the join adds partitions f, f + 8, ... in phase f, then the phases in order
 
-// CTAs of the first kernel that share an SM: the rings of 256 / head_dim of them fill its shared memory.
-__host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim) { return 256u / head_dim; }
-// The cut of a lane of n slots: one item for every resident CTA once the lane is long enough, at least 128 slots each.
+// CTAs of the first kernel that share an SM: their rings fill its shared memory, their accumulators its registers.  Several, so
+// that one streams while another joins its warps, fetches a query or looks up a page.
+__host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim, bool wide) { return head_dim == 256u ? 2u : head_dim == 128u && wide ? 3u : 4u; }
+// The cut of a lane of n slots: partitions of at least 128 slots, and no more items than one CTA for each SM (head_dim 256) or two
+// take in one go.  Fewer and longer ones serve a batch better (fewer records), more of them would only help a lane alone.
 __host__ __device__ inline uint32_t pd_per_wave(uint32_t kv_heads, uint32_t head_dim) {
-    const uint32_t p = kSmCount * pd_ctas(head_dim) / kv_heads;
+    const uint32_t p = kSmCount * (head_dim == 256u ? 1u : 2u) / kv_heads;
     return p == 0u ? 1u : p;
 }
 __host__ __device__ inline uint32_t pd_part_slots(uint32_t n, uint32_t per_wave) {
@@ -56,6 +58,8 @@ struct PagedDecodeParams {
     uint32_t n_lanes, max_keys, q_heads, group, per_wave;
     uint32_t parts;        // parts of the longest lane: the stride of sums and stats
     uint32_t score_slots;  // max_keys rounded up to 16
+    uint32_t units;        // places of a warp's ring
+    uint32_t page_slices, page_magic;   // slices of a page; floor(2^32 / page_slices) + 1
     float scale_log2e;
 };
 
@@ -85,10 +89,11 @@ template <> struct Half<__half> {
     static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__half*>(p) = __float2half_rn(v); }
 };
 
-// The items of every lane, counted by each CTA for itself: item_start[i] (n_lanes + 1 entries) and the lanes' slot
-// counts, 0 for a lane that is idle or refused.  Called by all threads.
-template <uint32_t kThreads>
-__device__ __forceinline__ void scan_items(const PagedDecodeParams& p, uint32_t* item_start, uint32_t* lane_keys, uint32_t* warp_total, bool latch) {
+// The work of every lane, counted by each CTA for itself: item_start[i] (n_lanes + 1 entries, count(slots) for each kv head) and
+// the lanes' slot counts, 0 for a lane that is idle or refused.  Called by all threads.
+template <uint32_t kThreads, typename Count>
+__device__ __forceinline__ void scan_items(const PagedDecodeParams& p, uint32_t* item_start, uint32_t* lane_keys, uint32_t* warp_total, bool latch,
+                                           Count count_of) {
     constexpr uint32_t kOwn = (TATARA_MAX_LANES + kThreads - 1u) / kThreads, kWarps = kThreads / 32u;
     const uint32_t first = threadIdx.x * kOwn, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     uint32_t mine = 0, count[kOwn];
@@ -104,7 +109,7 @@ __device__ __forceinline__ void scan_items(const PagedDecodeParams& p, uint32_t*
             }
             lane_keys[i] = n;
         }
-        count[j] = n == 0u ? 0u : pd_parts(n, p.per_wave) * p.cache.kv_heads;
+        count[j] = n == 0u ? 0u : count_of(n) * p.cache.kv_heads;
         mine += count[j];
     }
     uint32_t incl = mine;
@@ -131,13 +136,15 @@ __device__ __forceinline__ void scan_items(const PagedDecodeParams& p, uint32_t*
 struct PagedItem {
     uint32_t lane, kv, part, begin, slots;   // slots of the partition, from slot `begin` of the lane
 };
-__device__ __forceinline__ PagedItem item_at(const PagedDecodeParams& p, const uint32_t* item_start, const uint32_t* lane_keys, uint32_t item) {
+// Size(slots) is the length of a lane's pieces.
+template <typename Size>
+__device__ __forceinline__ PagedItem item_at(const PagedDecodeParams& p, const uint32_t* item_start, const uint32_t* lane_keys, uint32_t item, Size size_of) {
     uint32_t lo = 0, hi = p.n_lanes;   // last lane with item_start <= item (lanes without items share their successor's)
     while (hi - lo > 1u) {
         const uint32_t mid = (lo + hi) >> 1;
         if (item_start[mid] <= item) lo = mid; else hi = mid;
     }
-    const uint32_t local = item - item_start[lo], n = lane_keys[lo], size = pd_part_slots(n, p.per_wave);
+    const uint32_t local = item - item_start[lo], n = lane_keys[lo], size = size_of(n);
     PagedItem it;
     it.lane = lo;
     it.part = local / p.cache.kv_heads;
@@ -147,105 +154,175 @@ __device__ __forceinline__ PagedItem item_at(const PagedDecodeParams& p, const u
     return it;
 }
 
+constexpr uint32_t kPdItems = 128, kPdLookahead = 32;   // descriptors a CTA holds of its items; how far a warp reads ahead of its arithmetic
+
 template <int D>
 struct PdGeometry {
-    static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kSlice = kPagedSlice * kRow, kStage = 2 * kSlice;
-    static constexpr uint32_t kRing = kPdStages * kStage;                 // a warp's
-    static constexpr uint32_t kMergeRow = D + 4;                          // floats: the padding spreads the heads over the banks
-    static_assert(8 * kMergeRow * 4 <= kStage, "a warp's eight rows of the merge lie in one ring stage");
-    static constexpr uint32_t kSmem = kPdWarps * kRing + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 8) * 4;
+    static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kUnit = kPagedSlice * kRow;   // a unit: the K or the V rows of a slice
+    static constexpr uint32_t kMaxUnits = 6;
+    static constexpr uint32_t smem(uint32_t units) { return kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
+    // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and the rest of the SM's memory
+    // serves the copies better as L1 than as a deeper ring.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings an SM, 93 - 99 at
+    // 160 to 192; 32 lanes of 16384: 189 us at 128 KiB, 205 at 192.
+    static constexpr uint32_t units(uint32_t ctas) {
+        const uint32_t u = 1u + 64u * 1024u / (ctas * kPdWarps * kUnit);
+        return u < 2u ? 2u : u > kMaxUnits ? kMaxUnits : u;
+    }
+    static_assert(8 * D * 4 <= kUnit, "a warp's eight rows of the merge lie in one unit of its ring");
 };
+
+// 2^x; below 2^-126 zero
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // kTiles: tiles of eight query heads, 1 or 2.
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kPdThreads, pd_ctas(D))
+__global__ void __launch_bounds__(kPdThreads, pd_ctas(D, kTiles == 2))
 paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     using G = PdGeometry<D>;
     constexpr uint32_t kSteps = D / 16;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    float2* merge_ml = reinterpret_cast<float2*>(smem + kPdWarps * G::kRing);
+    uint4* items = reinterpret_cast<uint4*>(smem + kPdWarps * p.units * G::kUnit);    // {lane | kv << 16, part, begin, slots}
+    float2* merge_ml = reinterpret_cast<float2*>(items + kPdItems);
     uint32_t* item_start = reinterpret_cast<uint32_t*>(merge_ml + kPdWarps * 8);
     uint32_t* lane_keys = item_start + TATARA_MAX_LANES + 1;
-    uint32_t* warp_total = lane_keys + TATARA_MAX_LANES;
-    const uint32_t ring = smem_u32(smem + warp * G::kRing);
+    uint32_t* warp_word = lane_keys + TATARA_MAX_LANES;
+    const uint32_t ring = smem_u32(smem + warp * p.units * G::kUnit);
     const uint64_t policy = l2_evict_first_policy();
     wait_for_predecessor();
     release_dependents();
-    scan_items<kPdThreads>(p, item_start, lane_keys, warp_total, blockIdx.x == 0);
+    scan_items<kPdThreads>(p, item_start, lane_keys, warp_word, blockIdx.x == 0, [&](uint32_t n) { return pd_parts(n, p.per_wave); });
     const uint32_t total = item_start[p.n_lanes];
-
-    // ---- the warp's stream of slices, kPdStages - 1 ahead of the arithmetic, across items
-    uint32_t next_item = blockIdx.x, turn = 0, issued = 0, consumed = 0;
-    uint32_t pages = 0;            // lane j: page of the warp's slice 32 * (turn / 32) + j of the item
-    uint32_t absent = 0;           // bit s: the page of ring stage s does not exist
-    PagedItem pi{};
-    bool more = next_item < total;
-    if (more) pi = item_at(p, item_start, lane_keys, next_item);
+    // this CTA's items are blockIdx.x, blockIdx.x + gridDim.x, ...; a thread describes one
+    const uint32_t count = total > blockIdx.x ? (total - 1u - blockIdx.x) / gridDim.x + 1u : 0u;
+    auto describe = [&](uint32_t k) {
+        if (k >= count) return;
+        const PagedItem it = item_at(p, item_start, lane_keys, blockIdx.x + k * gridDim.x, [&](uint32_t n) { return pd_part_slots(n, p.per_wave); });
+        items[k % kPdItems] = make_uint4(it.lane | it.kv << 16, it.part, it.begin, it.slots);
+    };
+    describe(threadIdx.x);
+    __syncthreads();
+    // ---- the warp's stream of units, ahead of the arithmetic and across items: K and V of its slices in turn.
+    // pages, lane j: page of the warp's slice 32 * (turn / 32) + j of the item; the next item's are fetched an item early.
+    auto column_of = [&](uint32_t slice) { return p.page_slices == 1u ? slice : __umulhi(slice, p.page_magic); };   // of the lane's slice
+    auto fetch_pages = [&](const uint4& it, uint32_t from) {
+        const uint32_t slice = warp + (from + lane) * kPdWarps;
+        return slice * kPagedSlice < it.w
+                   ? __ldcg(p.cache.page_table + uint64_t(it.x & 0xFFFFu) * p.cache.table_pages + column_of(it.z / kPagedSlice + slice)) : 0u;
+    };
+    uint32_t at = 0, turn = 0, issued = 0, consumed = 0, done_items = 0, pages = 0, next_pages = 0;
+    uint32_t absent = 0;           // bit s: the page of the K unit in ring place s does not exist
+    uint4 pi = make_uint4(0u, 0u, 0u, 0u);
+    if (count != 0u) {
+        pi = items[0];
+        pages = fetch_pages(pi, 0u);
+        if (count > 1u) next_pages = fetch_pages(items[1], 0u);
+    }
+    uint32_t place_in = 0, place_out = 0;   // issued and consumed, modulo the ring's places
+    bool second = false;
+    uint64_t unit_offset = 0;
+    uint32_t unit_rows = 0;
+    const uint32_t chunk = lane % G::kChunks, row0 = lane / G::kChunks;
+    const uint64_t row_step = (32u / G::kChunks) * p.cache.slot_bytes;
+    // Asks for the next unit, if there is one and it may be asked for.
     auto issue = [&]() {
-        // the next slice of this warp: of the current item, or of the next item that has one for it
-        while (more && (warp + turn * kPdWarps) * kPagedSlice >= pi.slots) {
-            next_item += gridDim.x;
-            turn = 0;
-            more = next_item < total;
-            if (more) pi = item_at(p, item_start, lane_keys, next_item);
-        }
-        if (more) {
-            if ((turn & 31u) == 0u) {
-                const uint32_t slot = (warp + (turn + lane) * kPdWarps) * kPagedSlice;
-                if (slot < pi.slots) pages = __ldcg(p.cache.page_table + uint64_t(pi.lane) * p.cache.table_pages + (pi.begin + slot) / p.cache.page_slots);
+        if (!second) {
+            // the next slice of this warp: of the current item, or of the next item that has one for it
+            while (at < count && (warp + turn * kPdWarps) * kPagedSlice >= pi.w) {
+                if (at + 1u >= count) { at = count; break; }
+                if (at + 2u > done_items + kPdLookahead) return;
+                ++at;
+                turn = 0;
+                pi = items[at % kPdItems];
+                pages = next_pages;
+                if (at + 1u < count) next_pages = fetch_pages(items[(at + 1u) % kPdItems], 0u);
             }
+        }
+        if (at >= count) return;
+        const uint32_t place = place_in;
+        if (!second) {
+            if (turn != 0u && (turn & 31u) == 0u) pages = fetch_pages(pi, turn);
             const uint32_t page = __shfl_sync(0xffffffffu, pages, turn & 31u);
             const uint32_t first = (warp + turn * kPdWarps) * kPagedSlice;
+            const uint32_t slice = (pi.z + first) / kPagedSlice;
             const bool exists = page < p.cache.n_pages;
-            const uint32_t rows = exists ? min(kPagedSlice, pi.slots - first) : 0u;
-            const uint32_t stage = issued % kPdStages;
-            absent = (absent & ~(1u << stage)) | (exists ? 0u : 1u << stage);
-            if (!exists && lane == 0) latch_out_of_range(p.cache, pi.lane);
-            const uint64_t offset = exists ? page * p.cache.page_bytes + pi.kv * p.cache.head_bytes +
-                                                 ((pi.begin + first) % p.cache.page_slots) * p.cache.slot_bytes
-                                           : 0ull;
-            const uint32_t chunk = lane % G::kChunks, row0 = lane / G::kChunks;
-            const uint8_t* ksrc = p.cache.keys + offset + chunk * 16u;
-            const uint8_t* vsrc = p.cache.values + offset + chunk * 16u;
-            const uint32_t dst0 = ring + stage * G::kStage;
+            absent = (absent & ~(1u << place)) | (exists ? 0u : 1u << place);
+            if (!exists && lane == 0) latch_out_of_range(p.cache, pi.x & 0xFFFFu);
+            unit_rows = exists ? min(kPagedSlice, pi.w - first) : 0u;
+            unit_offset = exists ? page * p.cache.page_bytes + (pi.x >> 16) * p.cache.head_bytes +
+                                       (slice - column_of(slice) * p.page_slices) * kPagedSlice * p.cache.slot_bytes
+                                 : 0ull;
+            ++turn;
+        }
+        const uint8_t* src = (second ? p.cache.values : p.cache.keys) + unit_offset + chunk * 16u;
+        const uint32_t dst0 = ring + place * G::kUnit;
+        if (unit_rows == kPagedSlice) {
+            src += row0 * p.cache.slot_bytes;
 #pragma unroll
             for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
                 const uint32_t row = r + row0;
-                const bool live = row < rows;    // rows behind the partition and absent pages read nothing: zeros
-                const uint64_t off = live ? row * p.cache.slot_bytes : 0ull;
-                const uint32_t dst = dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4);
-                cp_async_16(dst, ksrc + off, live ? 16u : 0u, policy);
-                cp_async_16(dst + G::kSlice, vsrc + off, live ? 16u : 0u, policy);
+                cp_async_16(dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src, 16u, policy);
+                src += row_step;
             }
-            ++turn;
+        } else {
+#pragma unroll 1
+            for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
+                const uint32_t row = r + row0;
+                const bool live = row < unit_rows;    // rows behind the partition and absent pages read nothing: zeros
+                cp_async_16(dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src + (live ? row * p.cache.slot_bytes : 0ull), live ? 16u : 0u, policy);
+            }
         }
+        second = !second;
         cp_async_commit();
         ++issued;
+        place_in = place_in + 1u == p.units ? 0u : place_in + 1u;
     };
-#pragma unroll
-    for (uint32_t i = 0; i + 1 < kPdStages; ++i) issue();
+    // Waits for the oldest unit: all but the issued - consumed - 1 youngest groups have to be there.
+    auto await_unit = [&]() {
+        const uint32_t younger = issued - consumed - 1u;
+        if (younger == 1u) cp_async_wait<1>();
+        else if (younger == 2u) cp_async_wait<2>();
+        else if (younger == 0u) cp_async_wait<0>();
+        else if (younger == 3u) cp_async_wait<3>();
+        else if (younger == 4u) cp_async_wait<4>();
+        else cp_async_wait<5>();
+        __syncwarp();
+    };
+    auto release_unit = [&]() {
+        __syncwarp();   // every lane is done with this unit before it is refilled
+        ++consumed;
+        place_out = place_out + 1u == p.units ? 0u : place_out + 1u;
+    };
+#pragma unroll 1
+    for (uint32_t i = 1; i < p.units; ++i) issue();
 
     // Products run transposed, so that the 16 rows of the A operand are slots (scores) and dims (values) and the heads sit
-    // in the eight columns: S^T = K Q^T, O^T += V^T P^T.  A by ldmatrix out of the XOR-swizzled slice, Q and P^T in registers.
+    // in the eight columns: S^T = K Q^T, O^T += V^T P^T.  A by ldmatrix out of the XOR-swizzled unit, Q and P^T in registers.
     const uint32_t lm_j = lane >> 3, lm_r = lane & 7u;
     const uint32_t k_row = ((lm_j & 1u) * 8u + lm_r) * G::kRow, k_chunk = lm_j >> 1;
     const uint32_t v_row = ((lm_j >> 1) * 8u + lm_r) * G::kRow, v_chunk = lm_j & 1u;
 
-    for (uint32_t item = blockIdx.x; item < total; item += gridDim.x) {
-        const PagedItem ci = item_at(p, item_start, lane_keys, item);
-        uint32_t qf[kTiles][kSteps][2];
+    uint32_t qf[kTiles][kSteps][2];
+    auto load_query = [&](const uint4& it) {
 #pragma unroll
         for (uint32_t nt = 0; nt < kTiles; ++nt) {
             const uint32_t head = nt * 8u + g;
             const uint32_t* row = reinterpret_cast<const uint32_t*>(
-                p.q + (ci.lane * p.query_stride + uint64_t(ci.kv * p.group + (head < p.group ? head : 0u)) * D) * 2u);
+                p.q + ((it.x & 0xFFFFu) * p.query_stride + uint64_t((it.x >> 16) * p.group + (head < p.group ? head : 0u)) * D) * 2u);
 #pragma unroll
             for (uint32_t ks = 0; ks < kSteps; ++ks) {
                 qf[nt][ks][0] = head < p.group ? __ldcg(row + ks * 8u + t) : 0u;
                 qf[nt][ks][1] = head < p.group ? __ldcg(row + ks * 8u + 4u + t) : 0u;
             }
         }
+    };
+    uint4 ci = pi;
+    if (count != 0u) load_query(ci);
+    while (done_items < count) {
         float o[kTiles][kSteps][4], m[kTiles][2], l[kTiles][2];
 #pragma unroll
         for (uint32_t nt = 0; nt < kTiles; ++nt) {
@@ -254,16 +331,15 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.0f;
         }
+        const uint32_t slots = ci.w;
         float* score_base = p.scores == nullptr ? nullptr
-                            : p.scores + ((uint64_t(ci.lane) * p.cache.kv_heads + ci.kv) * p.score_slots + ci.begin) * (kTiles * 8u);
+                            : p.scores + ((uint64_t(ci.x & 0xFFFFu) * p.cache.kv_heads + (ci.x >> 16)) * p.score_slots + ci.z) * (kTiles * 8u);
 
-        for (uint32_t slice = warp; slice * kPagedSlice < ci.slots; slice += kPdWarps) {
-            issue();
-            cp_async_wait<kPdStages - 1>();
-            __syncwarp();
-            const uint32_t stage = consumed % kPdStages;
-            const uint32_t kst = ring + stage * G::kStage, vst = kst + G::kSlice;
-            const bool exists = ((absent >> stage) & 1u) == 0u;
+        for (uint32_t first = warp * kPagedSlice; first < slots; first += kPdWarps * kPagedSlice) {
+            if (issued - consumed < p.units) issue();
+            await_unit();
+            const uint32_t kst = ring + place_out * G::kUnit;
+            const bool exists = ((absent >> place_out) & 1u) == 0u;
             float s[kTiles][4], s2[kTiles][4];
 #pragma unroll
             for (uint32_t nt = 0; nt < kTiles; ++nt)
@@ -279,69 +355,90 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 #pragma unroll
                 for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s2[nt], a0, a1, a2, a3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
             }
+            release_unit();
+            issue();
             // lane (g, t): slots g and g + 8 of the slice, heads 2t and 2t + 1 of each tile
-            const uint32_t slot0 = slice * kPagedSlice + g;
-            const bool live0 = exists && slot0 < ci.slots, live1 = exists && slot0 + 8u < ci.slots;
-            float alpha[kTiles][2];
-            uint32_t pb[kTiles][2];
-            bool rescale = false;
+            const bool live0 = exists && first + g < slots, live1 = exists && first + g + 8u < slots;
+            float x[kTiles][4];
+            bool higher = false;
 #pragma unroll
             for (uint32_t nt = 0; nt < kTiles; ++nt) {
-                float x[4];
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) x[i] = (i < 2 ? live0 : live1) ? (s[nt][i] + s2[nt][i]) * p.scale_log2e : -INFINITY;
-                if (score_base != nullptr) {
-                    float* at = score_base + uint64_t(slot0) * (kTiles * 8u) + nt * 8u + 2u * t;
-                    if (slot0 < ci.slots) *reinterpret_cast<float2*>(at) = make_float2(x[0], x[1]);
-                    if (slot0 + 8u < ci.slots) *reinterpret_cast<float2*>(at + 8u * kTiles * 8u) = make_float2(x[2], x[3]);
-                }
-                float mx0 = fmaxf(x[0], x[2]), mx1 = fmaxf(x[1], x[3]);
+                for (uint32_t i = 0; i < 4; ++i) x[nt][i] = (i < 2 ? live0 : live1) ? (s[nt][i] + s2[nt][i]) * p.scale_log2e : -INFINITY;
+                higher = higher || x[nt][0] > m[nt][0] || x[nt][2] > m[nt][0] || x[nt][1] > m[nt][1] || x[nt][3] > m[nt][1];
+            }
+            if (score_base != nullptr) {
 #pragma unroll
-                for (uint32_t off = 4; off < 32; off <<= 1) {
-                    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
-                    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+                for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                    float* to = score_base + uint64_t(first + g) * (kTiles * 8u) + nt * 8u + 2u * t;
+                    if (first + g < slots) *reinterpret_cast<float2*>(to) = make_float2(x[nt][0], x[nt][1]);
+                    if (first + g + 8u < slots) *reinterpret_cast<float2*>(to + 8u * kTiles * 8u) = make_float2(x[nt][2], x[nt][3]);
                 }
-                const float n0 = fmaxf(m[nt][0], mx0), n1 = fmaxf(m[nt][1], mx1);
-                // nothing seen yet (an absent page, scores of -inf): every weight is 2^(-inf) = 0 against any finite base
-                const float b0 = n0 == -INFINITY ? 0.0f : n0, b1 = n1 == -INFINITY ? 0.0f : n1;
-                alpha[nt][0] = exp2f(m[nt][0] - b0);
-                alpha[nt][1] = exp2f(m[nt][1] - b1);
-                const float p0 = exp2f(x[0] - b0), p1 = exp2f(x[1] - b1), p2 = exp2f(x[2] - b0), p3 = exp2f(x[3] - b1);
-                l[nt][0] = l[nt][0] * alpha[nt][0] + (p0 + p2);
-                l[nt][1] = l[nt][1] * alpha[nt][1] + (p1 + p3);
-                m[nt][0] = n0;
-                m[nt][1] = n1;
+            }
+            // The maximum rises a few times at the start of an item and hardly ever later: only then is it looked for across the slice's
+            // slots and everything summed so far scaled down.
+            if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+                for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                    float mx0 = fmaxf(x[nt][0], x[nt][2]), mx1 = fmaxf(x[nt][1], x[nt][3]);
+#pragma unroll
+                    for (uint32_t off = 4; off < 32; off <<= 1) {
+                        mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
+                        mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, off));
+                    }
+                    mx0 = fmaxf(m[nt][0], mx0);
+                    mx1 = fmaxf(m[nt][1], mx1);
+                    // (a column still at -inf has no sum yet: its factor 2^(-inf) is 0 against any finite base)
+                    const float a0 = exp2_fast(m[nt][0] - (mx0 == -INFINITY ? 0.0f : mx0)), a1 = exp2_fast(m[nt][1] - (mx1 == -INFINITY ? 0.0f : mx1));
+                    m[nt][0] = mx0;
+                    m[nt][1] = mx1;
+                    l[nt][0] *= a0;
+                    l[nt][1] *= a1;
+#pragma unroll
+                    for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                        o[nt][ks][0] *= a0;
+                        o[nt][ks][1] *= a1;
+                        o[nt][ks][2] *= a0;
+                        o[nt][ks][3] *= a1;
+                    }
+                }
+            }
+            uint32_t pb[kTiles][2];
+#pragma unroll
+            for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+                const float p0 = exp2_fast(x[nt][0] - b0), p1 = exp2_fast(x[nt][1] - b1), p2 = exp2_fast(x[nt][2] - b0), p3 = exp2_fast(x[nt][3] - b1);
+                l[nt][0] += p0 + p2;
+                l[nt][1] += p1 + p3;
                 // the weights are rounded to the cache's type for the second product: half a step each, of random sign
                 pb[nt][0] = movmatrix_trans(Half<T>::pack(p0, p1));   // slots 2t, 2t+1 of head g
                 pb[nt][1] = movmatrix_trans(Half<T>::pack(p2, p3));   // slots 2t+8, 2t+9 of head g
-                rescale = rescale || alpha[nt][0] != 1.0f || alpha[nt][1] != 1.0f;
             }
-            // a factor of exactly 1 leaves every bit as it is, so the rescale is skipped when no lane needs it
-            rescale = __any_sync(0xffffffffu, rescale);
+            await_unit();
+            const uint32_t vst = ring + place_out * G::kUnit;
 #pragma unroll
             for (uint32_t ks = 0; ks < kSteps; ++ks) {
                 uint32_t a0, a1, a2, a3;
                 ldmatrix_x4_trans(vst + v_row + (((ks * 2u + v_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
 #pragma unroll
-                for (uint32_t nt = 0; nt < kTiles; ++nt) {
-                    if (rescale) {
-                        o[nt][ks][0] *= alpha[nt][0];
-                        o[nt][ks][1] *= alpha[nt][1];
-                        o[nt][ks][2] *= alpha[nt][0];
-                        o[nt][ks][3] *= alpha[nt][1];
-                    }
-                    Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-                }
+                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
             }
-            __syncwarp();   // every lane is done with this stage before it is refilled
-            ++consumed;
+            release_unit();
         }
 
-        // ---- the four warps' parts of the item, joined eight heads at a time.  Each warp lays its rows over the ring stage
-        // that it read last: kPdStages - 1 stages are in flight or waiting, so that one is free until the next issue().
-        const uint32_t free_stage = (consumed + kPdStages - 1u) % kPdStages;
-        float* merge_mine = reinterpret_cast<float*>(smem + warp * G::kRing + free_stage * G::kStage);
-        if (lane == 0) warp_total[warp] = free_stage;
+        // the next item's query is on its way while this item's warps are joined
+        const uint4 done = ci;
+        ++done_items;
+        if (done_items < count) {
+            ci = items[done_items % kPdItems];
+            load_query(ci);
+        }
+        // ---- the four warps' parts of the item, joined eight heads at a time.  Each warp lays its rows over the unit of its ring
+        // that it read last: the others are in flight or waiting, that one is free until the next issue().  Dims are
+        // XORed with a multiple of 8 by head so that the four heads that a warp stores at once fall into different banks.
+        const uint32_t free_place = place_out == 0u ? p.units - 1u : place_out - 1u;
+        float* merge_mine = reinterpret_cast<float*>(smem + (warp * p.units + free_place) * G::kUnit);
+        if (lane == 0) warp_word[warp] = free_place;
 #pragma unroll
         for (uint32_t nt = 0; nt < kTiles; ++nt) {
 #pragma unroll
@@ -349,13 +446,16 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                 l[nt][0] += __shfl_xor_sync(0xffffffffu, l[nt][0], off);
                 l[nt][1] += __shfl_xor_sync(0xffffffffu, l[nt][1], off);
             }
-            float* mo = merge_mine + 2u * t * G::kMergeRow + g;
+            float* mo = merge_mine + 2u * t * D;
+            if (nt * 8u + 2u * t < p.group) {
 #pragma unroll
-            for (uint32_t ks = 0; ks < kSteps; ++ks) {
-                mo[ks * 16u] = o[nt][ks][0];
-                mo[G::kMergeRow + ks * 16u] = o[nt][ks][1];
-                mo[ks * 16u + 8u] = o[nt][ks][2];
-                mo[G::kMergeRow + ks * 16u + 8u] = o[nt][ks][3];
+                for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                    const uint32_t d0 = (ks * 16u + g) ^ (t << 3), d1 = (ks * 16u + 8u + g) ^ (t << 3);
+                    mo[d0] = o[nt][ks][0];
+                    mo[D + d0] = o[nt][ks][1];
+                    mo[d1] = o[nt][ks][2];
+                    mo[D + d1] = o[nt][ks][3];
+                }
             }
             if (g == 0) {
                 merge_ml[warp * 8u + 2u * t] = make_float2(m[nt][0], l[nt][0]);
@@ -370,18 +470,18 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 #pragma unroll
                 for (uint32_t w = 0; w < kPdWarps; ++w) {
                     const float2 ml = merge_ml[w * 8u + h];
-                    wt[w] = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+                    wt[w] = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - top);
                     sum = fmaf(wt[w], ml.y, sum);
                 }
-                const uint64_t record = (uint64_t(ci.lane) * p.q_heads + ci.kv * p.group + head) * p.parts + ci.part;
+                const uint64_t record = (uint64_t(done.x & 0xFFFFu) * p.q_heads + (done.x >> 16) * p.group + head) * p.parts + done.y;
                 float4* dst = reinterpret_cast<float4*>(p.sums + record * D);
 #pragma unroll
                 for (uint32_t d4 = threadIdx.x & 15u; d4 < D / 4; d4 += 16u) {
                     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                     for (uint32_t w = 0; w < kPdWarps; ++w) {
-                        const float4 v = *reinterpret_cast<const float4*>(smem + w * G::kRing + warp_total[w] * G::kStage +
-                                                                          (h * G::kMergeRow + d4 * 4u) * 4u);
+                        const float4 v = *reinterpret_cast<const float4*>(smem + (w * p.units + warp_word[w]) * G::kUnit +
+                                                                          (h * D + ((d4 * 4u) ^ ((h >> 1) << 3))) * 4u);
                         acc.x = fmaf(wt[w], v.x, acc.x);
                         acc.y = fmaf(wt[w], v.y, acc.y);
                         acc.z = fmaf(wt[w], v.z, acc.z);
@@ -391,6 +491,9 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                 }
                 if ((threadIdx.x & 15u) == 0u) p.stats[record] = make_float2(top, sum);
             }
+            // half of the descriptors lie behind every warp: the half after the other one takes their place
+            if (nt + 1u == kTiles && done_items % (kPdItems / 2u) == 0u && threadIdx.x < kPdItems / 2u)
+                describe(done_items + kPdItems / 2u + threadIdx.x);
             __syncthreads();
         }
     }
@@ -398,22 +501,24 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 }
 
 // ---- the join -----------------------------------------------------------------------------
-// CTAs 0 .. lanes*q_heads*D/64 - 1 finish 64 dims of a head each; the others walk the items again and add the weights to the mass.
+// With a mass, the first `walkers` CTAs add the weights to it, kMassSpan slots of a kv head at a time; the others finish 64 dims of a
+// head each.
+constexpr uint32_t kMassSpan = 1024;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads)
-paged_join_kernel(const __grid_constant__ PagedDecodeParams p) {
+paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t walkers) {
     __shared__ uint32_t item_start[TATARA_MAX_LANES + 1], lane_keys[TATARA_MAX_LANES], warp_total[kJoinWarps];
-    __shared__ float weight[kSmCount * 4];                 // at most per_wave partitions
+    __shared__ float weight[kSmCount * 2];                 // per_wave at most
     __shared__ float red[kJoinWarps];
     __shared__ __align__(16) float acc_s[kJoinPhases][kJoinDims];
     __shared__ float2 final_ml[16];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     constexpr uint32_t kSlices = D / kJoinDims;
-    const uint32_t pieces = p.n_lanes * p.q_heads * kSlices;
     wait_for_predecessor();
     release_dependents();
-    if (blockIdx.x < pieces) {
-        const uint32_t slice = blockIdx.x % kSlices, rest = blockIdx.x / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
+    if (blockIdx.x >= walkers) {
+        const uint32_t piece = blockIdx.x - walkers, slice = piece % kSlices, rest = piece / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
         const uint32_t n = __ldcg(&p.lanes[row].keys);
         if (n > p.max_keys) return;                        // refused: its row stays as it is
         const uint32_t parts = n == 0u ? 0u : pd_parts(n, p.per_wave);
@@ -480,40 +585,67 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p) {
         }
         return;
     }
-    scan_items<kJoinThreads>(p, item_start, lane_keys, warp_total, false);
+    scan_items<kJoinThreads>(p, item_start, lane_keys, warp_total, false, [](uint32_t n) { return (n + kMassSpan - 1u) / kMassSpan; });
     const uint32_t total = item_start[p.n_lanes], row_floats = (p.group + 7u) / 8u * 8u;
-    for (uint32_t item = blockIdx.x - pieces; item < total; item += gridDim.x - pieces) {
-        const PagedItem it = item_at(p, item_start, lane_keys, item);
+    for (uint32_t item = blockIdx.x; item < total; item += walkers) {
+        const PagedItem it = item_at(p, item_start, lane_keys, item, [](uint32_t) { return kMassSpan; });
         const uint32_t parts = pd_parts(lane_keys[it.lane], p.per_wave);
+        const uint64_t head_row = uint64_t(it.lane) * p.cache.kv_heads + it.kv;
+        const float* scores = p.scores + (head_row * p.score_slots + it.begin) * row_floats;
+        float* mass = p.cache.mass + head_row * p.cache.capacity + it.begin;
+        // the heads' maximum and the reciprocal of their sum
         for (uint32_t h = warp; h < p.group; h += kJoinWarps) {
             const float2* st = p.stats + (uint64_t(it.lane) * p.q_heads + it.kv * p.group + h) * p.parts;
             float top = -INFINITY, sum = 0.0f;
-            for (uint32_t part = lane; part < parts; part += 32u) top = fmaxf(top, __ldcg(&st[part]).x);
+            for (uint32_t part0 = 0; part0 < parts; part0 += 160u) {
+                float2 ml[5];
+                float big = top;
 #pragma unroll
-            for (uint32_t off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            for (uint32_t part = lane; part < parts; part += 32u) {
-                const float2 ml = __ldcg(&st[part]);
-                sum = fmaf(ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top), ml.y, sum);
+                for (uint32_t i = 0; i < 5; ++i) {
+                    const uint32_t part = part0 + i * 32u + lane;
+                    ml[i] = part < parts ? __ldcg(&st[part]) : make_float2(-INFINITY, 0.0f);
+                    big = fmaxf(big, ml[i].x);
+                }
+#pragma unroll
+                for (uint32_t off = 16; off; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+                sum *= top == -INFINITY ? 0.0f : exp2f(top - big);
+#pragma unroll
+                for (uint32_t i = 0; i < 5; ++i) sum = fmaf(ml[i].x == -INFINITY ? 0.0f : exp2f(ml[i].x - big), ml[i].y, sum);
+                top = big;
             }
 #pragma unroll
             for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
             if (lane == 0) final_ml[h] = make_float2(top == -INFINITY ? 0.0f : top, sum == 0.0f ? 0.0f : 1.0f / sum);
         }
         __syncthreads();
-        const uint64_t head_row = uint64_t(it.lane) * p.cache.kv_heads + it.kv;
-        const float* scores = p.scores + (head_row * p.score_slots + it.begin) * row_floats;
-        float* mass = p.cache.mass + head_row * p.cache.capacity + it.begin;
-        for (uint32_t slot = threadIdx.x; slot < it.slots; slot += kJoinThreads) {
-            const float* x = scores + uint64_t(slot) * row_floats;
-            float w = 0.0f;
-            for (uint32_t h0 = 0; h0 < p.group; h0 += 4u) {
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(x + h0));
-                const float e[4] = {v.x, v.y, v.z, v.w};
+        constexpr uint32_t kOwn = kMassSpan / kJoinThreads;
+        float w[kOwn], before[kOwn];
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j)
-                    if (h0 + j < p.group) w = fmaf(exp2f(e[j] - final_ml[h0 + j].x), final_ml[h0 + j].y, w);
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            const uint32_t slot = i * kJoinThreads + threadIdx.x;
+            before[i] = slot < it.slots ? __ldcg(mass + slot) : 0.0f;
+            w[i] = 0.0f;
+        }
+        for (uint32_t h0 = 0; h0 < p.group; h0 += 4u) {
+            float4 v[kOwn];
+#pragma unroll
+            for (uint32_t i = 0; i < kOwn; ++i) {
+                const uint32_t slot = i * kJoinThreads + threadIdx.x;
+                v[i] = __ldcg(reinterpret_cast<const float4*>(scores + uint64_t(slot < it.slots ? slot : 0u) * row_floats + h0));
             }
-            mass[slot] += w;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                if (h0 + j >= p.group) break;
+                const float2 ml = final_ml[h0 + j];
+#pragma unroll
+                for (uint32_t i = 0; i < kOwn; ++i)
+                    w[i] = fmaf(exp2f((j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w) - ml.x), ml.y, w[i]);
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kOwn; ++i) {
+            const uint32_t slot = i * kJoinThreads + threadIdx.x;
+            if (slot < it.slots) mass[slot] = before[i] + w[i];
         }
         __syncthreads();
     }
@@ -539,22 +671,25 @@ static PagedDecodeLayout pd_layout(const tatara_paged_cache& c, uint32_t n_lanes
 }
 
 template <typename T, int D, int kTiles>
-static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, const PagedDecodeParams& p) {
+static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, PagedDecodeParams p) {
+    using G = PdGeometry<D>;
+    constexpr uint32_t kCtas = pd_ctas(D, kTiles == 2);
     static bool configured[64] = {false};
     if (!configured[ctx->device & 63]) {
-        if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 PdGeometry<D>::kSmem) != cudaSuccess)
+        if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(G::units(1u))) != cudaSuccess)
             return check_launch(ctx, "attn_decode_paged: shared memory attribute");
         configured[ctx->device & 63] = true;
     }
-    const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, resident = uint64_t(ctx->sm_count) * pd_ctas(D);
-    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < resident ? items : resident)), kPdThreads,
-                        PdGeometry<D>::kSmem, stream, p);
+    const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, sms = ctx->sm_count;
+    const uint32_t ctas = items >= kCtas * sms ? kCtas : uint32_t((items + sms - 1u) / sms);   // on an SM
+    p.units = G::units(ctas);
+    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < kCtas * sms ? items : kCtas * sms)), kPdThreads, G::smem(p.units), stream, p);
     const tatara_status st = check_launch(ctx, "attn_decode_paged");
     if (st != TATARA_OK) return st;
     const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
-    const uint64_t walkers = p.cache.mass == nullptr ? 0u : items < 4u * ctx->sm_count ? items : 4u * ctx->sm_count;
-    (void)launch_staged(paged_join_kernel<T, D>, dim3(pieces + uint32_t(walkers)), kJoinThreads, 0u, stream, p);
+    const uint64_t spans = uint64_t(p.n_lanes) * p.cache.kv_heads * ((p.max_keys + kMassSpan - 1u) / kMassSpan);
+    const uint32_t walkers = p.cache.mass == nullptr ? 0u : uint32_t(spans < 4u * ctx->sm_count ? spans : 4u * ctx->sm_count);
+    (void)launch_staged(paged_join_kernel<T, D>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
     return check_launch(ctx, "attn_decode_paged: join");
 }
 
@@ -614,6 +749,8 @@ extern "C" tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream,
     p.per_wave = l.per_wave;
     p.parts = l.parts;
     p.score_slots = l.score_slots;
+    p.page_slices = cache->page_slots / kPagedSlice;
+    p.page_magic = uint32_t((1ull << 32) / p.page_slices) + 1u;   // (a single slice to a page is taken apart: 2^32 does not fit)
     p.scale_log2e = scale * kPdLog2e;
     const DeviceGuard guard(ctx);
     return cache->dtype == TATARA_BF16 ? pick_paged_decode<__nv_bfloat16>(ctx, static_cast<cudaStream_t>(stream), p, cache->head_dim)
