@@ -6,10 +6,10 @@
 // does not ask for an order of the slots, so nothing else moves: 8 x head_dim bytes for each pair against the whole kept part
 // for a cache that is kept in order.
 //
-// Two launches.  paged_select_kernel finds the keep-th key by a radix search (11 + 11 + 10 bits) and writes the two lists;
-// one cluster of CTAs holds the keys of a head in shared memory, so that mass and positions are read once and the histograms are added
-// over distributed shared memory.  paged_move_kernel copies the rows.  Bound: HBM (the rows) for a large cut,
-// latency of the search for a small one.
+// Two launches.  paged_select_kernel finds the keep-th key by a radix search (11 + 11 + 10 bits) and writes the two lists: up
+// to 16 keys sit in the registers of each thread, so mass and positions are read once, and up to 16 CTAs of a cluster share a head
+// and add their histograms over distributed shared memory.  paged_move_kernel copies the rows.  Bound: HBM (the rows) for a
+// large cut, the latency of the search's steps for a small one.
 #include "paged.cuh"
 
 #include <cooperative_groups.h>
@@ -18,9 +18,9 @@ namespace tb {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kSelThreads = 512, kSelWarps = kSelThreads / 32, kSelBins = 2048, kSelMaxCluster = 8;
-constexpr uint32_t kSelMaxChunk = 49152;                 // keys of one CTA: 192 KiB beside the three histograms
-constexpr uint32_t kMoveThreads = 256;
+constexpr uint32_t kSelThreads = 1024, kSelWarps = kSelThreads / 32, kSelBins = 2048, kSelMaxCluster = 16, kSelMaxKeys = 16;
+static_assert(kSelThreads * kSelMaxKeys * kSelMaxCluster >= TATARA_MAX_CONTEXT, "one cluster holds the longest lane");
+constexpr uint32_t kMoveThreads = 256, kMoveBatch = 4;
 
 struct PagedEvictParams {
     PagedView cache;
@@ -30,15 +30,18 @@ struct PagedEvictParams {
     uint32_t* donors;    // [row][room]
     uint32_t n_lanes, max_keys, keep, sink, recent;
     uint32_t room;       // no row has more pairs
-    uint32_t cluster, chunk;
-    uint32_t move_blocks, move_pairs;   // blocks of the second kernel for each row, pairs of a block
+    uint32_t cluster;
+    uint32_t move_blocks, warp_pairs;   // blocks of the second kernel for each row, pairs of a warp (at most 32)
 };
 
 struct SelectShared {
     uint32_t hist[3][kSelBins];
-    uint32_t ties, holes, donors;                        // of this CTA, read by the others of the cluster
-    uint32_t warp_a[kSelWarps], warp_b[kSelWarps];
-    uint32_t bin, above;                                 // the digit that holds the threshold, keys beyond it
+    uint4 warp_counts[kSelWarps];
+    uint4 counts;                    // of this CTA, read by the others of the cluster
+    uint32_t slice[kSelBins];        // this CTA's share of the cluster's bins, summed up from the top; read by the others
+    uint32_t slice_total[kSelMaxCluster];   // of every CTA, written by each
+    uint32_t warp_sum[kSelWarps];
+    uint32_t bin, above;             // the digit that holds the threshold, keys beyond it
 };
 
 // An unsigned integer in the order of the floats: negative ones reversed, not-a-number first, the guarded slots' value left free.
@@ -48,38 +51,25 @@ __device__ __forceinline__ uint32_t rank_key(float mass) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ uint32_t block_exclusive(uint32_t mine, uint32_t* warp_sum, uint32_t& total) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    uint32_t incl = mine;
+__device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
 #pragma unroll
     for (uint32_t off = 1; off < 32; off <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, off);
-        if (lane >= off) incl += v;
+        const uint32_t u = __shfl_up_sync(0xffffffffu, v, off);
+        if ((threadIdx.x & 31u) >= off) v += u;
     }
-    __syncthreads();
-    if (lane == 31u) warp_sum[warp] = incl;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kSelWarps; ++w) {
-        if (w < warp) before += warp_sum[w];
-        total += warp_sum[w];
-    }
-    return before + incl - mine;
+    return v;
 }
 
+// kKeys: keys of a thread.  A warp owns a run of 32 kKeys slots, lane by lane, so ballots count in the order of the slots.
+template <uint32_t kKeys>
 __global__ void __launch_bounds__(kSelThreads, 1)
 paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
-    extern __shared__ __align__(16) uint8_t sel_smem[];
-    SelectShared& s = *reinterpret_cast<SelectShared*>(sel_smem);
-    uint32_t* keys = reinterpret_cast<uint32_t*>(sel_smem + sizeof(SelectShared));
+    __shared__ __align__(16) SelectShared s;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
     const uint32_t lane_row = row / p.cache.kv_heads, head = row - lane_row * p.cache.kv_heads;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     for (uint32_t i = threadIdx.x; i < 3u * kSelBins; i += kSelThreads) (&s.hist[0][0])[i] = 0u;
-    if (threadIdx.x == 0) s.ties = s.holes = s.donors = 0u;
     wait_for_predecessor();
     release_dependents();
     const uint2 l = __ldcg(reinterpret_cast<const uint2*>(p.lanes + lane_row));   // keys, position
@@ -89,140 +79,233 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
         if (rank == 0u && threadIdx.x == 0) p.counts[row] = 0u;
         return;
     }
-    __syncthreads();
-    const uint32_t base = rank * p.chunk, mine = base >= n ? 0u : min(p.chunk, n - base);
-    const uint64_t plane = plane_row(p.cache, lane_row, head) + base;
+    const uint32_t unit = rank * kSelThreads * kKeys + warp * 32u * kKeys, first = unit + lane;   // the thread's slots: first + 32 j
+    const uint64_t plane = plane_row(p.cache, lane_row, head);
 
-    // ---- keys into shared memory, with the first digit's histogram
-#pragma unroll 4
-    for (uint32_t i = threadIdx.x; i < mine; i += kSelThreads) {
-        const float mass = __ldcg(p.cache.mass + plane + i);
-        bool guarded = base + i < p.sink;
-        if (p.recent != 0u) guarded = guarded || uint64_t(__ldcg(p.cache.positions + plane + i)) + p.recent > l.y;
-        const uint32_t key = guarded ? 0xFFFFFFFFu : rank_key(mass);
-        keys[i] = key;
-        atomicAdd(&s.hist[0][key >> 21], 1u);
+    // ---- keys into registers; a slot that is not there gets no key
+    uint32_t key[kKeys];
+    {
+        float mass[kKeys];
+        uint32_t where[kKeys];
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            const uint32_t slot = first + 32u * j;
+            mass[j] = slot < n ? __ldcg(p.cache.mass + plane + slot) : 0.0f;
+        }
+        if (p.recent != 0u) {
+#pragma unroll
+            for (uint32_t j = 0; j < kKeys; ++j) {
+                const uint32_t slot = first + 32u * j;
+                where[j] = slot < n ? __ldcg(p.cache.positions + plane + slot) : 0u;
+            }
+        }
+        const uint32_t newest = p.recent > l.y ? 0u : l.y - p.recent + 1u;   // positions from here on are guarded
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            const bool guarded = first + 32u * j < p.sink || (p.recent != 0u && where[j] >= newest);
+            key[j] = guarded ? 0xFFFFFFFFu : rank_key(mass[j]);
+        }
     }
+    __syncthreads();
 
     // ---- radix search: the digits of the keep-th largest key, the largest digit first
     uint32_t prefix = 0u, want = p.keep;     // `want` keys are still to be found among those with this prefix
 #pragma unroll
     for (uint32_t digit = 0; digit < 3u; ++digit) {
         const uint32_t shift = digit == 0u ? 21u : digit == 1u ? 10u : 0u, bins = digit == 2u ? 1024u : 2048u;
-        if (digit != 0u) {
-            const uint32_t upper = digit == 1u ? 21u : 10u;
-            for (uint32_t i = threadIdx.x; i < mine; i += kSelThreads) {
-                const uint32_t key = keys[i];
-                if (key >> upper == prefix) atomicAdd(&s.hist[digit][(key >> shift) & (bins - 1u)], 1u);
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            const bool in = first + 32u * j < n && (digit == 0u || key[j] >> (digit == 1u ? 21u : 10u) == prefix);
+            const uint32_t bin = (key[j] >> shift) & (bins - 1u);
+            // (a run of guarded, untouched or equal slots falls into one bin: one addition for all of them)
+            const bool full = __all_sync(0xffffffffu, in);
+            const uint32_t its = __shfl_sync(0xffffffffu, bin, 0);
+            if (full && __all_sync(0xffffffffu, bin == its)) {
+                if (lane == 0u) atomicAdd(&s.hist[digit][bin], 32u);
+            } else if (in) {
+                atomicAdd(&s.hist[digit][bin], 1u);
             }
         }
         cluster.sync();
-        // thread t adds up the cluster's bins 4t .. 4t+3, counted from the top
-        uint32_t c[4] = {0u, 0u, 0u, 0u};
-        const uint32_t top = bins - 4u - threadIdx.x * 4u;
-        const bool holds = threadIdx.x * 4u < bins;
-        if (holds) {
-            for (uint32_t r = 0; r < p.cluster; ++r) {
-                const uint4 v = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(&s.hist[digit][top], r));
-                c[0] += v.w; c[1] += v.z; c[2] += v.y; c[3] += v.x;
+        if (p.cluster == 1u) {
+            // thread t takes bins 2t and 2t + 1, counted from the top
+            const uint32_t top = bins - 2u - threadIdx.x * 2u;
+            const bool holds = threadIdx.x * 2u < bins;
+            uint2 v = make_uint2(0u, 0u);
+            if (holds) v = *reinterpret_cast<const uint2*>(&s.hist[digit][top]);
+            const uint32_t incl = warp_inclusive(v.x + v.y);
+            if (lane == 31u) s.warp_sum[warp] = incl;
+            __syncthreads();
+            const uint32_t sums = warp_inclusive(s.warp_sum[lane]);
+            const uint32_t before = __shfl_sync(0xffffffffu, sums, warp == 0u ? 0u : warp - 1u);
+            const uint32_t above = (warp == 0u ? 0u : before) + incl - v.x - v.y;
+            if (holds && above < want && want <= above + v.x + v.y) {
+                const bool upper = want <= above + v.y;
+                s.bin = top + (upper ? 1u : 0u);
+                s.above = upper ? above : above + v.y;
             }
-        }
-        uint32_t total;
-        uint32_t above = block_exclusive(c[0] + c[1] + c[2] + c[3], s.warp_a, total);
-        if (holds) {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                if (above < want && want <= above + c[j]) {
-                    s.bin = bins - 1u - (threadIdx.x * 4u + j);
-                    s.above = above;
+        } else {
+            // Each CTA adds up one slice of the bins over the cluster (the slice of rank 0 is the topmost), sums it up from the top and
+            // tells the others its total: a few hundred bytes cross between SMs in place of every histogram to every CTA.
+            const uint32_t width = bins / p.cluster, slice_top = bins - 1u - rank * width;
+            uint32_t mine = 0u;
+            if (threadIdx.x < width)
+                for (uint32_t r = 0; r < p.cluster; ++r) mine += *cluster.map_shared_rank(&s.hist[digit][slice_top - threadIdx.x], r);
+            const uint32_t incl = warp_inclusive(mine);
+            if (lane == 31u) s.warp_sum[warp] = incl;
+            __syncthreads();
+            const uint32_t sums = warp_inclusive(s.warp_sum[lane]);
+            const uint32_t before = __shfl_sync(0xffffffffu, sums, warp == 0u ? 0u : warp - 1u);
+            if (threadIdx.x < width) s.slice[threadIdx.x] = (warp == 0u ? 0u : before) + incl;
+            const uint32_t all = __shfl_sync(0xffffffffu, sums, 31);
+            if (threadIdx.x < p.cluster) *cluster.map_shared_rank(&s.slice_total[rank], threadIdx.x) = all;
+            cluster.sync();
+            const uint32_t of_rank = warp_inclusive(lane < p.cluster ? s.slice_total[lane] : 0u);
+            const uint32_t owner = __ffs(__ballot_sync(0xffffffffu, want <= of_rank)) - 1u;       // (the last rank's sum is at least `want`)
+            const uint32_t over = __shfl_sync(0xffffffffu, of_rank, owner == 0u ? 0u : owner - 1u);
+            const uint32_t above = owner == 0u ? 0u : over;
+            if (threadIdx.x < width) {
+                const uint32_t to = above + *cluster.map_shared_rank(&s.slice[threadIdx.x], owner);
+                const uint32_t from = threadIdx.x == 0u ? above : above + *cluster.map_shared_rank(&s.slice[threadIdx.x - 1u], owner);
+                if (from < want && want <= to) {
+                    s.bin = bins - 1u - owner * width - threadIdx.x;
+                    s.above = from;
                 }
-                above += c[j];
             }
         }
         __syncthreads();
         prefix = digit == 0u ? s.bin : (prefix << (digit == 1u ? 11 : 10)) | s.bin;
         want -= s.above;
-        __syncthreads();
     }
-    // keys above `prefix` stay; of those equal to it the first `want`, by slot
 
-    // ---- which stay: each warp owns a run of the chunk, in slot order
-    const uint32_t run = (p.chunk / kSelWarps + 31u) / 32u * 32u, run0 = min(mine, warp * run), run1 = min(mine, run0 + run);
-    uint32_t ties = 0u;
-    for (uint32_t i = run0 + lane; i < run1; i += 32u) ties += keys[i] == prefix ? 1u : 0u;
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    uint32_t total, tie_rank = block_exclusive(lane == 0u ? ties : 0u, s.warp_a, total);
-    tie_rank = __shfl_sync(0xffffffffu, tie_rank, 0);
-    if (threadIdx.x == 0) s.ties = total;
+    // ---- keys above `prefix` stay, and of those equal to it the first `want` by slot.  Four counts of every warp, below slot `keep` (x, y)
+    // and from it on (z, w), those above and those equal, give each warp its place in both lists.
+    uint32_t low_counts = 0u, high_counts = 0u;   // those above | those equal << 16
+#pragma unroll
+    for (uint32_t j = 0; j < kKeys; ++j) {
+        const uint32_t slot = first + 32u * j;
+        const uint32_t one = slot >= n || key[j] < prefix ? 0u : key[j] == prefix ? 0x10000u : 1u;
+        low_counts += slot < p.keep ? one : 0u;
+        high_counts += slot < p.keep ? 0u : one;
+    }
+    low_counts = __reduce_add_sync(0xffffffffu, low_counts);
+    high_counts = __reduce_add_sync(0xffffffffu, high_counts);
+    const uint4 c = make_uint4(low_counts & 0xFFFFu, low_counts >> 16, high_counts & 0xFFFFu, high_counts >> 16);
+    if (lane == 0u) s.warp_counts[warp] = c;
+    __syncthreads();
+    const uint4 of = s.warp_counts[lane];
+    const uint4 sum = make_uint4(warp_inclusive(of.x), warp_inclusive(of.y), warp_inclusive(of.z), warp_inclusive(of.w));
+    if (threadIdx.x == 31u) s.counts = sum;
+    const uint32_t prior = warp == 0u ? 0u : warp - 1u;
+    uint4 b = make_uint4(__shfl_sync(0xffffffffu, sum.x, prior), __shfl_sync(0xffffffffu, sum.y, prior), __shfl_sync(0xffffffffu, sum.z, prior),
+                         __shfl_sync(0xffffffffu, sum.w, prior));
+    if (warp == 0u) b = make_uint4(0u, 0u, 0u, 0u);
     cluster.sync();
-    for (uint32_t r = 0; r < rank; ++r) tie_rank += *cluster.map_shared_rank(&s.ties, r);
-    uint32_t holes = 0u, donors = 0u;
-    for (uint32_t i0 = run0; i0 < run1; i0 += 32u) {
-        const uint32_t i = i0 + lane;
-        const uint32_t key = i < run1 ? keys[i] : 0u;
-        const bool tie = i < run1 && key == prefix;
-        const uint32_t tied = __ballot_sync(0xffffffffu, tie);
-        const bool kept = i < run1 && (key > prefix || (tie && tie_rank + __popc(tied & ((1u << lane) - 1u)) < want));
-        tie_rank += __popc(tied);
-        const bool low = base + i < p.keep;
-        if (i < run1) keys[i] = low ? (kept ? 0u : 1u) : (kept ? 2u : 0u);   // 1: hole, 2: donor
-        holes += __popc(__ballot_sync(0xffffffffu, i < run1 && low && !kept));
-        donors += __popc(__ballot_sync(0xffffffffu, i < run1 && !low && kept));
+    const uint4 other = lane < p.cluster ? *cluster.map_shared_rank(&s.counts, lane) : make_uint4(0u, 0u, 0u, 0u);
+    const bool prior_rank = lane < rank;
+    b.x += __reduce_add_sync(0xffffffffu, prior_rank ? other.x : 0u);
+    b.y += __reduce_add_sync(0xffffffffu, prior_rank ? other.y : 0u);
+    b.z += __reduce_add_sync(0xffffffffu, prior_rank ? other.z : 0u);
+    b.w += __reduce_add_sync(0xffffffffu, prior_rank ? other.w : 0u);
+    if (rank == 0u && warp == 0u) {
+        const uint32_t over = __reduce_add_sync(0xffffffffu, other.x), ties = __reduce_add_sync(0xffffffffu, other.y);
+        if (lane == 0u) p.counts[row] = p.keep - over - min(want, ties);
     }
-    uint32_t hole_total, donor_total;
-    uint32_t hole_at = block_exclusive(lane == 0u ? holes : 0u, s.warp_a, hole_total);
-    uint32_t donor_at = block_exclusive(lane == 0u ? donors : 0u, s.warp_b, donor_total);
-    hole_at = __shfl_sync(0xffffffffu, hole_at, 0);
-    donor_at = __shfl_sync(0xffffffffu, donor_at, 0);
-    if (threadIdx.x == 0) {
-        s.holes = hole_total;
-        s.donors = donor_total;
-    }
-    cluster.sync();
-    uint32_t hole_sum = 0u;
-    for (uint32_t r = 0; r < p.cluster; ++r) {
-        const uint32_t h = *cluster.map_shared_rank(&s.holes, r);
-        if (r < rank) {
-            hole_at += h;
-            donor_at += *cluster.map_shared_rank(&s.donors, r);
-        }
-        hole_sum += h;
-    }
-    if (rank == 0u && threadIdx.x == 0) p.counts[row] = hole_sum;
+    // ties below `keep` come before those from it on, so the first `want` of all are min(want, y) below and the rest above
+    uint32_t tie_rank = b.y + b.w;
+    uint32_t hole_at = min(p.keep, unit) - b.x - min(want, b.y), donor_at = b.z + min(want, b.y + b.w) - min(want, b.y);
     uint32_t* hole_list = p.holes + uint64_t(row) * p.room;
     uint32_t* donor_list = p.donors + uint64_t(row) * p.room;
-    for (uint32_t i0 = run0; i0 < run1; i0 += 32u) {
-        const uint32_t i = i0 + lane, mark = i < run1 ? keys[i] : 0u, below = (1u << lane) - 1u;
-        const uint32_t hb = __ballot_sync(0xffffffffu, mark == 1u), db = __ballot_sync(0xffffffffu, mark == 2u);
-        const uint32_t h = hole_at + __popc(hb & below), d = donor_at + __popc(db & below);
-        if (mark == 1u && h < p.room) hole_list[h] = base + i;
-        if (mark == 2u && d < p.room) donor_list[d] = base + i;
-        hole_at += __popc(hb);
-        donor_at += __popc(db);
+    const uint32_t below = (1u << lane) - 1u;
+    const bool all_ties = tie_rank + c.y + c.w <= want, split = !all_ties && tie_rank < want;   // what of the warp's ties stays: all, some, none
+    if (!split && unit + 32u * kKeys <= p.keep) {
+        // the warp's slots all lie below `keep`: holes only
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            const bool hole = key[j] < prefix || (!all_ties && key[j] == prefix);
+            const uint32_t hb = __ballot_sync(0xffffffffu, hole), h = hole_at + __popc(hb & below);
+            if (hole && h < p.room) hole_list[h] = first + 32u * j;
+            hole_at += __popc(hb);
+        }
+    } else if (!split && unit >= p.keep) {
+        // or from it on: donors only
+#pragma unroll
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            const bool donor = first + 32u * j < n && (key[j] > prefix || (all_ties && key[j] == prefix));
+            const uint32_t db = __ballot_sync(0xffffffffu, donor), d = donor_at + __popc(db & below);
+            if (donor && d < p.room) donor_list[d] = first + 32u * j;
+            donor_at += __popc(db);
+        }
+    } else {
+#pragma unroll 1
+        for (uint32_t j = 0; j < kKeys; ++j) {
+            uint32_t mine = key[0];
+#pragma unroll
+            for (uint32_t i = 1; i < kKeys; ++i) mine = i == j ? key[i] : mine;
+            const uint32_t slot = first + 32u * j;
+            const bool tie = slot < n && mine == prefix;
+            const uint32_t tied = __ballot_sync(0xffffffffu, tie);
+            const bool kept = slot < n && (mine > prefix || (tie && tie_rank + __popc(tied & below) < want));
+            tie_rank += __popc(tied);
+            const bool hole = slot < p.keep && !kept, donor = slot >= p.keep && kept;       // (slots below `keep` all exist: n > keep)
+            const uint32_t hb = __ballot_sync(0xffffffffu, hole), db = __ballot_sync(0xffffffffu, donor);
+            const uint32_t h = hole_at + __popc(hb & below), d = donor_at + __popc(db & below);
+            if (hole && h < p.room) hole_list[h] = slot;
+            if (donor && d < p.room) donor_list[d] = slot;
+            hole_at += __popc(hb);
+            donor_at += __popc(db);
+        }
     }
     cluster.sync();   // nobody leaves while its counters are read
 }
 
+// A warp takes p.warp_pairs pairs: each lane looks up one pair's slots and pages, then kChunks lanes together copy a pair's rows, with
+// the loads of kMoveBatch steps on their way before the first store.
 template <uint32_t kChunks>   // 16-byte chunks of a row
 __global__ void __launch_bounds__(kMoveThreads)
 paged_move_kernel(const __grid_constant__ PagedEvictParams p) {
+    constexpr uint32_t kTogether = 32u / kChunks;   // pairs of a step
     const uint32_t row = blockIdx.x / p.move_blocks, block = blockIdx.x - row * p.move_blocks;
-    const uint32_t lane_row = row / p.cache.kv_heads, head = row - lane_row * p.cache.kv_heads;
+    const uint32_t lane_row = row / p.cache.kv_heads, head = row - lane_row * p.cache.kv_heads, lane = threadIdx.x & 31u;
     wait_for_predecessor();
-    const uint32_t pairs = __ldcg(p.counts + row), first = block * p.move_pairs, last = min(pairs, first + p.move_pairs);
-    const uint64_t plane = plane_row(p.cache, lane_row, head);
-    const uint32_t chunk = threadIdx.x % kChunks;
-    for (uint32_t j = first + threadIdx.x / kChunks; j < last; j += kMoveThreads / kChunks) {
-        const uint32_t to = __ldcg(p.holes + uint64_t(row) * p.room + j), from = __ldcg(p.donors + uint64_t(row) * p.room + j);
-        uint64_t src, dst;
-        if (!slot_offset(p.cache, lane_row, head, from, src) || !slot_offset(p.cache, lane_row, head, to, dst)) continue;
-        const uint4 k = __ldcs(reinterpret_cast<const uint4*>(p.cache.keys + src + chunk * 16u));
-        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p.cache.values + src + chunk * 16u));
-        *reinterpret_cast<uint4*>(p.cache.keys + dst + chunk * 16u) = k;
-        *reinterpret_cast<uint4*>(p.cache.values + dst + chunk * 16u) = v;
-        if (chunk == 0u) {
+    const uint32_t pairs = __ldcg(p.counts + row), first = (block * (kMoveThreads / 32u) + (threadIdx.x >> 5)) * p.warp_pairs;
+    if (first >= pairs) return;
+    const uint32_t mine = min(p.warp_pairs, pairs - first);
+    uint64_t src = 0, dst = 0;
+    uint32_t ok = 0u;
+    if (lane < mine) {
+        const uint64_t at = uint64_t(row) * p.room + first + lane;
+        const uint32_t to = __ldcg(p.holes + at), from = __ldcg(p.donors + at);
+        const bool there = slot_offset(p.cache, lane_row, head, from, src);
+        if (slot_offset(p.cache, lane_row, head, to, dst) && there) {
+            ok = 1u;
+            const uint64_t plane = plane_row(p.cache, lane_row, head);
             p.cache.mass[plane + to] = __ldcg(p.cache.mass + plane + from);
             if (p.cache.positions != nullptr) p.cache.positions[plane + to] = __ldcg(p.cache.positions + plane + from);
+        }
+    }
+    const uint32_t sub = lane / kChunks, offset = (lane % kChunks) * 16u;
+    for (uint32_t j0 = 0; j0 < mine; j0 += kMoveBatch * kTogether) {
+        uint4 k[kMoveBatch], v[kMoveBatch];
+        uint64_t to[kMoveBatch];
+        bool live[kMoveBatch];
+#pragma unroll
+        for (uint32_t i = 0; i < kMoveBatch; ++i) {
+            const uint32_t j = j0 + i * kTogether + sub;
+            const uint64_t from = __shfl_sync(0xffffffffu, src, j & 31u) + offset;
+            to[i] = __shfl_sync(0xffffffffu, dst, j & 31u) + offset;
+            live[i] = (__shfl_sync(0xffffffffu, ok, j & 31u) & (j < mine ? 1u : 0u)) != 0u;
+            if (live[i]) {
+                k[i] = __ldcs(reinterpret_cast<const uint4*>(p.cache.keys + from));
+                v[i] = __ldcs(reinterpret_cast<const uint4*>(p.cache.values + from));
+            }
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kMoveBatch; ++i) {
+            if (live[i]) {
+                *reinterpret_cast<uint4*>(p.cache.keys + to[i]) = k[i];
+                *reinterpret_cast<uint4*>(p.cache.values + to[i]) = v[i];
+            }
         }
     }
 }
@@ -269,22 +352,22 @@ extern "C" tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const
     p.counts = static_cast<uint32_t*>(scratch);
     p.holes = p.counts + (rows * 4u + 255u) / 256u * 64u;
     p.donors = p.holes + rows * p.room;
-    // CTAs of a cluster: as few as hold the keys, more while SMs are idle and there is something to share.
+    // As few CTAs as hold a head's keys 16 to a thread: below 16384 slots none has to wait for another.
     p.cluster = 1u;
-    while (p.cluster < kSelMaxCluster &&
-           ((max_keys + p.cluster - 1u) / p.cluster > kSelMaxChunk ||
-            (rows * p.cluster * 2u <= uint64_t(ctx->sm_count) && max_keys / p.cluster > 2048u)))
-        p.cluster *= 2u;
-    p.chunk = ((max_keys + p.cluster - 1u) / p.cluster + 511u) / 512u * 512u;
-    p.move_pairs = 4u * kMoveThreads / (cache->head_dim / 8u);
-    p.move_blocks = (p.room + p.move_pairs - 1u) / p.move_pairs;
+    while (p.cluster * kSelThreads * kSelMaxKeys < max_keys) p.cluster *= 2u;
+    const uint32_t keys = (max_keys + p.cluster * kSelThreads - 1u) / (p.cluster * kSelThreads);   // of a thread
+    auto select = keys <= 2u ? paged_select_kernel<2> : keys <= 4u ? paged_select_kernel<4> : keys <= 8u ? paged_select_kernel<8> : paged_select_kernel<16>;
+    // A few pairs go to many warps, many pairs 32 to a warp: one look-up for all lanes.
+    const uint64_t spread = rows * p.room / (uint64_t(ctx->sm_count) * 32u);
+    p.warp_pairs = spread < 4u ? 4u : spread > 32u ? 32u : uint32_t(spread);
+    const uint32_t block_pairs = kMoveThreads / 32u * p.warp_pairs;
+    p.move_blocks = (p.room + block_pairs - 1u) / block_pairs;
     if (rows * p.move_blocks > 0x7FFFFFFFull) return fail(ctx, TATARA_INVALID_DISPATCH_EXTENT, "paged_evict: grid");
     const DeviceGuard guard(ctx);
     static bool configured[64] = {false};
     if (!configured[ctx->device & 63]) {
-        if (cudaFuncSetAttribute(paged_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 sizeof(SelectShared) + kSelMaxChunk * 4u) != cudaSuccess)
-            return check_launch(ctx, "paged_evict: shared memory attribute");
+        if (cudaFuncSetAttribute(paged_select_kernel<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+            return check_launch(ctx, "paged_evict: cluster attribute");
         configured[ctx->device & 63] = true;
     }
     cudaLaunchAttribute attr[2];
@@ -297,11 +380,10 @@ extern "C" tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(uint32_t(rows * p.cluster));
     cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = sizeof(SelectShared) + p.chunk * 4u;
     cfg.stream = static_cast<cudaStream_t>(stream);
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    (void)cudaLaunchKernelEx(&cfg, paged_select_kernel, p);
+    (void)cudaLaunchKernelEx(&cfg, select, p);
     const tatara_status launched = check_launch(ctx, "paged_evict");
     if (launched != TATARA_OK) return launched;
     auto move = cache->head_dim == 64u ? paged_move_kernel<8> : cache->head_dim == 128u ? paged_move_kernel<16> : paged_move_kernel<32>;
