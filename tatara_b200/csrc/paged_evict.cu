@@ -60,7 +60,8 @@ __device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
     return v;
 }
 
-// kKeys: keys of a thread.  A warp owns a run of 32 kKeys slots, lane by lane, so ballots count in the order of the slots.
+// kKeys: the most keys of a thread; `each` of them are used, as many as the lane's slots need.  A warp owns a run of 32 * each slots,
+// lane by lane, so ballots count in the order of the slots.
 template <uint32_t kKeys>
 __global__ void __launch_bounds__(kSelThreads, 1)
 paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
@@ -79,7 +80,8 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
         if (rank == 0u && threadIdx.x == 0) p.counts[row] = 0u;
         return;
     }
-    const uint32_t unit = rank * kSelThreads * kKeys + warp * 32u * kKeys, first = unit + lane;   // the thread's slots: first + 32 j
+    const uint32_t each = (n + p.cluster * kSelThreads - 1u) / (p.cluster * kSelThreads);
+    const uint32_t unit = (rank * kSelWarps + warp) * 32u * each, first = unit + lane;            // the thread's slots: first + 32 j
     const uint64_t plane = plane_row(p.cache, lane_row, head);
 
     // ---- keys into registers; a slot that is not there gets no key
@@ -90,18 +92,21 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
 #pragma unroll
         for (uint32_t j = 0; j < kKeys; ++j) {
             const uint32_t slot = first + 32u * j;
+            if (j >= each) break;
             mass[j] = slot < n ? __ldcg(p.cache.mass + plane + slot) : 0.0f;
         }
         if (p.recent != 0u) {
 #pragma unroll
             for (uint32_t j = 0; j < kKeys; ++j) {
                 const uint32_t slot = first + 32u * j;
+                if (j >= each) break;
                 where[j] = slot < n ? __ldcg(p.cache.positions + plane + slot) : 0u;
             }
         }
         const uint32_t newest = p.recent > l.y ? 0u : l.y - p.recent + 1u;   // positions from here on are guarded
 #pragma unroll
         for (uint32_t j = 0; j < kKeys; ++j) {
+            if (j >= each) break;
             const bool guarded = first + 32u * j < p.sink || (p.recent != 0u && where[j] >= newest);
             key[j] = guarded ? 0xFFFFFFFFu : rank_key(mass[j]);
         }
@@ -115,6 +120,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
         const uint32_t shift = digit == 0u ? 21u : digit == 1u ? 10u : 0u, bins = digit == 2u ? 1024u : 2048u;
 #pragma unroll
         for (uint32_t j = 0; j < kKeys; ++j) {
+            if (j >= each) break;
             const bool in = first + 32u * j < n && (digit == 0u || key[j] >> (digit == 1u ? 21u : 10u) == prefix);
             const uint32_t bin = (key[j] >> shift) & (bins - 1u);
             // (a run of guarded, untouched or equal slots falls into one bin: one addition for all of them)
@@ -184,6 +190,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
 #pragma unroll
     for (uint32_t j = 0; j < kKeys; ++j) {
         const uint32_t slot = first + 32u * j;
+        if (j >= each) break;
         const uint32_t one = slot >= n || key[j] < prefix ? 0u : key[j] == prefix ? 0x10000u : 1u;
         low_counts += slot < p.keep ? one : 0u;
         high_counts += slot < p.keep ? 0u : one;
@@ -218,10 +225,11 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
     uint32_t* donor_list = p.donors + uint64_t(row) * p.room;
     const uint32_t below = (1u << lane) - 1u;
     const bool all_ties = tie_rank + c.y + c.w <= want, split = !all_ties && tie_rank < want;   // what of the warp's ties stays: all, some, none
-    if (!split && unit + 32u * kKeys <= p.keep) {
+    if (!split && unit + 32u * each <= p.keep) {
         // the warp's slots all lie below `keep`: holes only
 #pragma unroll
         for (uint32_t j = 0; j < kKeys; ++j) {
+            if (j >= each) break;
             const bool hole = key[j] < prefix || (!all_ties && key[j] == prefix);
             const uint32_t hb = __ballot_sync(0xffffffffu, hole), h = hole_at + __popc(hb & below);
             if (hole && h < p.room) hole_list[h] = first + 32u * j;
@@ -231,6 +239,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
         // or from it on: donors only
 #pragma unroll
         for (uint32_t j = 0; j < kKeys; ++j) {
+            if (j >= each) break;
             const bool donor = first + 32u * j < n && (key[j] > prefix || (all_ties && key[j] == prefix));
             const uint32_t db = __ballot_sync(0xffffffffu, donor), d = donor_at + __popc(db & below);
             if (donor && d < p.room) donor_list[d] = first + 32u * j;
@@ -238,7 +247,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
         }
     } else {
 #pragma unroll 1
-        for (uint32_t j = 0; j < kKeys; ++j) {
+        for (uint32_t j = 0; j < each; ++j) {
             uint32_t mine = key[0];
 #pragma unroll
             for (uint32_t i = 1; i < kKeys; ++i) mine = i == j ? key[i] : mine;
@@ -355,7 +364,7 @@ extern "C" tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const
     // As few CTAs as hold a head's keys 16 to a thread: below 16384 slots none has to wait for another.
     p.cluster = 1u;
     while (p.cluster * kSelThreads * kSelMaxKeys < max_keys) p.cluster *= 2u;
-    const uint32_t keys = (max_keys + p.cluster * kSelThreads - 1u) / (p.cluster * kSelThreads);   // of a thread
+    const uint32_t keys = (max_keys + p.cluster * kSelThreads - 1u) / (p.cluster * kSelThreads);   // of a thread, at most
     auto select = keys <= 2u ? paged_select_kernel<2> : keys <= 4u ? paged_select_kernel<4> : keys <= 8u ? paged_select_kernel<8> : paged_select_kernel<16>;
     // A few pairs go to many warps, many pairs 32 to a warp: one look-up for all lanes.
     const uint64_t spread = rows * p.room / (uint64_t(ctx->sm_count) * 32u);
