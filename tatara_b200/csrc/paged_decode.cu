@@ -158,7 +158,9 @@ constexpr uint32_t kPdItems = 128, kPdLookahead = 32;   // descriptors a CTA hol
 
 template <int D>
 struct PdGeometry {
-    static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kUnit = kPagedSlice * kRow;   // a unit: the K or the V rows of a slice
+    // A unit is the K or the V rows of a step: one slice, or two where rows are short (what a step costs beside its rows weighs more there).
+    static constexpr uint32_t kSlices = D == 64 ? 2 : 1, kStep = kSlices * kPagedSlice;
+    static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kUnit = kStep * kRow;
     static constexpr uint32_t kMaxUnits = 6;
     static constexpr uint32_t smem(uint32_t units) { return kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
     // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and the rest of the SM's memory
@@ -183,7 +185,7 @@ template <typename T, int D, int kTiles>
 __global__ void __launch_bounds__(kPdThreads, pd_ctas(D, kTiles == 2))
 paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     using G = PdGeometry<D>;
-    constexpr uint32_t kSteps = D / 16;
+    constexpr uint32_t kSteps = D / 16, kR = G::kSlices, kStep = G::kStep;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
     uint4* items = reinterpret_cast<uint4*>(smem + kPdWarps * p.units * G::kUnit);    // {lane | kv << 16, part, begin, slots}
@@ -207,73 +209,98 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     describe(threadIdx.x);
     __syncthreads();
     // ---- the warp's stream of units, ahead of the arithmetic and across items: K and V of its slices in turn.
-    // pages, lane j: page of the warp's slice 32 * (turn / 32) + j of the item; the next item's are fetched an item early.
+    // Lane j looks after slice j % kR of the warp's steps kTurns * (turn / kTurns) + j / kR of an item: it fetches the slice's page, for the
+    // next item an item early, and works out where the slice's rows lie; a step takes its slices' places from those lanes.
+    constexpr uint32_t kTurns = 32u / kR;
     auto column_of = [&](uint32_t slice) { return p.page_slices == 1u ? slice : __umulhi(slice, p.page_magic); };   // of the lane's slice
     auto fetch_pages = [&](const uint4& it, uint32_t from) {
-        const uint32_t slice = warp + (from + lane) * kPdWarps;
+        const uint32_t slice = (warp + (from + lane / kR) * kPdWarps) * kR + lane % kR;
         return slice * kPagedSlice < it.w
                    ? __ldcg(p.cache.page_table + uint64_t(it.x & 0xFFFFu) * p.cache.table_pages + column_of(it.z / kPagedSlice + slice)) : 0u;
     };
-    uint32_t at = 0, turn = 0, issued = 0, consumed = 0, done_items = 0, pages = 0, next_pages = 0;
-    uint32_t absent = 0;           // bit s: the page of the K unit in ring place s does not exist
+    uint64_t places = 0;
+    uint32_t missing = 0;          // bit j: lane j's page does not exist
+    auto settle = [&](const uint4& it, uint32_t from, uint32_t page) {
+        const uint32_t slice = (warp + (from + lane / kR) * kPdWarps) * kR + lane % kR, whole = it.z / kPagedSlice + slice;
+        places = page * p.cache.page_bytes + (it.x >> 16) * p.cache.head_bytes + (whole - column_of(whole) * p.page_slices) * kPagedSlice * p.cache.slot_bytes;
+        const bool none = slice * kPagedSlice < it.w && page >= p.cache.n_pages;
+        missing = __ballot_sync(0xffffffffu, none);
+        if (none) {
+            places = 0;
+            latch_out_of_range(p.cache, it.x & 0xFFFFu);
+        }
+    };
+    uint32_t at = 0, turn = 0, issued = 0, consumed = 0, done_items = 0, next_pages = 0;
+    uint32_t absent = 0;           // bits kR s ..: the pages of the K unit in ring place s that do not exist
     uint4 pi = make_uint4(0u, 0u, 0u, 0u);
     if (count != 0u) {
         pi = items[0];
-        pages = fetch_pages(pi, 0u);
+        settle(pi, 0u, fetch_pages(pi, 0u));
         if (count > 1u) next_pages = fetch_pages(items[1], 0u);
     }
     uint32_t place_in = 0, place_out = 0;   // issued and consumed, modulo the ring's places
+    uint32_t unit_place = 0;                // place of the K unit of the step under way
     bool second = false;
-    uint64_t unit_offset = 0;
-    uint32_t unit_rows = 0;
+    uint64_t unit_offset[kR] = {};
+    uint32_t unit_rows = 0;        // of the unit; slices of absent pages hold none
+    bool unit_whole = false;
     const uint32_t chunk = lane % G::kChunks, row0 = lane / G::kChunks;
     const uint64_t row_step = (32u / G::kChunks) * p.cache.slot_bytes;
     // Asks for the next unit, if there is one and it may be asked for.
     auto issue = [&]() {
         if (!second) {
             // the next slice of this warp: of the current item, or of the next item that has one for it
-            while (at < count && (warp + turn * kPdWarps) * kPagedSlice >= pi.w) {
+            while (at < count && (warp + turn * kPdWarps) * kStep >= pi.w) {
                 if (at + 1u >= count) { at = count; break; }
                 if (at + 2u > done_items + kPdLookahead) return;
                 ++at;
                 turn = 0;
                 pi = items[at % kPdItems];
-                pages = next_pages;
+                settle(pi, 0u, next_pages);
                 if (at + 1u < count) next_pages = fetch_pages(items[(at + 1u) % kPdItems], 0u);
             }
         }
         if (at >= count) return;
         const uint32_t place = place_in;
         if (!second) {
-            if (turn != 0u && (turn & 31u) == 0u) pages = fetch_pages(pi, turn);
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, turn & 31u);
-            const uint32_t first = (warp + turn * kPdWarps) * kPagedSlice;
-            const uint32_t slice = (pi.z + first) / kPagedSlice;
-            const bool exists = page < p.cache.n_pages;
-            absent = (absent & ~(1u << place)) | (exists ? 0u : 1u << place);
-            if (!exists && lane == 0) latch_out_of_range(p.cache, pi.x & 0xFFFFu);
-            unit_rows = exists ? min(kPagedSlice, pi.w - first) : 0u;
-            unit_offset = exists ? page * p.cache.page_bytes + (pi.x >> 16) * p.cache.head_bytes +
-                                       (slice - column_of(slice) * p.page_slices) * kPagedSlice * p.cache.slot_bytes
-                                 : 0ull;
+            unit_place = place;
+            if (turn != 0u && turn % kTurns == 0u) settle(pi, turn, fetch_pages(pi, turn));
+            const uint32_t from = turn % kTurns * kR, gone = (missing >> from) & ((1u << kR) - 1u);
+            unit_rows = min(kStep, pi.w - (warp + turn * kPdWarps) * kStep);
+            unit_whole = unit_rows == kStep && gone == 0u;
+            absent = (absent & ~(((1u << kR) - 1u) << (place * kR))) | gone << (place * kR);
+#pragma unroll
+            for (uint32_t i = 0; i < kR; ++i) unit_offset[i] = __shfl_sync(0xffffffffu, places, from + i);
             ++turn;
         }
-        const uint8_t* src = (second ? p.cache.values : p.cache.keys) + unit_offset + chunk * 16u;
+        const uint8_t* pool = (second ? p.cache.values : p.cache.keys) + chunk * 16u + row0 * p.cache.slot_bytes;
         const uint32_t dst0 = ring + place * G::kUnit;
-        if (unit_rows == kPagedSlice) {
-            src += row0 * p.cache.slot_bytes;
 #pragma unroll
-            for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
-                const uint32_t row = r + row0;
-                cp_async_16(dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src, 16u, policy);
-                src += row_step;
-            }
-        } else {
+        for (uint32_t i = 0; i < kR; ++i) {
+            const uint8_t* src = pool + unit_offset[i];
+            const uint32_t dst1 = dst0 + i * kPagedSlice * G::kRow;
+            if (unit_whole && p.cache.slot_bytes == G::kRow) {
+#pragma unroll
+                for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
+                    const uint32_t row = r + row0;
+                    cp_async_16(dst1 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src + r * G::kRow, 16u, policy);
+                }
+            } else if (unit_whole) {
+#pragma unroll
+                for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
+                    const uint32_t row = r + row0;
+                    cp_async_16(dst1 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src, 16u, policy);
+                    src += row_step;
+                }
+            } else {
 #pragma unroll 1
-            for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
-                const uint32_t row = r + row0;
-                const bool live = row < unit_rows;    // rows behind the partition and absent pages read nothing: zeros
-                cp_async_16(dst0 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), src + (live ? row * p.cache.slot_bytes : 0ull), live ? 16u : 0u, policy);
+                for (uint32_t r = 0; r < kPagedSlice; r += 32u / G::kChunks) {
+                    const uint32_t row = r + row0;
+                    // rows behind the partition and absent pages read nothing: zeros
+                    const bool live = i * kPagedSlice + row < unit_rows && ((absent >> (unit_place * kR + i)) & 1u) == 0u;
+                    cp_async_16(dst1 + row * G::kRow + ((chunk ^ (row & 7u)) << 4), live ? src : pool, live ? 16u : 0u, policy);
+                    src += row_step;
+                }
             }
         }
         second = !second;
@@ -335,52 +362,67 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
         float* score_base = p.scores == nullptr ? nullptr
                             : p.scores + ((uint64_t(ci.x & 0xFFFFu) * p.cache.kv_heads + (ci.x >> 16)) * p.score_slots + ci.z) * (kTiles * 8u);
 
-        for (uint32_t first = warp * kPagedSlice; first < slots; first += kPdWarps * kPagedSlice) {
+        for (uint32_t first = warp * kStep; first < slots; first += kPdWarps * kStep) {
             if (issued - consumed < p.units) issue();
             await_unit();
-            const uint32_t kst = ring + place_out * G::kUnit;
-            const bool exists = ((absent >> place_out) & 1u) == 0u;
-            float s[kTiles][4], s2[kTiles][4];
+            const uint32_t kst = ring + place_out * G::kUnit + k_row;
+            const uint32_t gone = absent >> (place_out * kR);
+            float s[kR][kTiles][4], s2[kR][kTiles][4];
 #pragma unroll
-            for (uint32_t nt = 0; nt < kTiles; ++nt)
+            for (uint32_t i = 0; i < kR; ++i) {
 #pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) s[nt][i] = s2[nt][i] = 0.0f;
+                for (uint32_t nt = 0; nt < kTiles; ++nt)
 #pragma unroll
-            for (uint32_t ks = 0; ks < kSteps; ks += 2) {
-                uint32_t a0, a1, a2, a3;
-                ldmatrix_x4(kst + k_row + (((ks * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+                    for (uint32_t e = 0; e < 4; ++e) s[i][nt][e] = s2[i][nt][e] = 0.0f;
 #pragma unroll
-                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s[nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1]);
-                ldmatrix_x4(kst + k_row + ((((ks + 1u) * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+                for (uint32_t ks = 0; ks < kSteps; ks += 2) {
+                    uint32_t a0, a1, a2, a3;
+                    // (the swizzle only touches the low three bits of a chunk: every fourth step shares its offset)
+                    ldmatrix_x4(kst + i * kPagedSlice * G::kRow + ks / 4u * 128u + (((ks % 4u * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
 #pragma unroll
-                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s2[nt], a0, a1, a2, a3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s[i][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1]);
+                    ldmatrix_x4(kst + i * kPagedSlice * G::kRow + ks / 4u * 128u + ((((ks + 1u) % 4u * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+#pragma unroll
+                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s2[i][nt], a0, a1, a2, a3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+                }
             }
             release_unit();
             issue();
-            // lane (g, t): slots g and g + 8 of the slice, heads 2t and 2t + 1 of each tile
-            const bool live0 = exists && first + g < slots, live1 = exists && first + g + 8u < slots;
-            float x[kTiles][4];
+            // lane (g, t): slots g and g + 8 of each slice, heads 2t and 2t + 1 of each tile
             bool higher = false;
 #pragma unroll
-            for (uint32_t nt = 0; nt < kTiles; ++nt) {
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) x[nt][i] = (i < 2 ? live0 : live1) ? (s[nt][i] + s2[nt][i]) * p.scale_log2e : -INFINITY;
-                higher = higher || x[nt][0] > m[nt][0] || x[nt][2] > m[nt][0] || x[nt][1] > m[nt][1] || x[nt][3] > m[nt][1];
-            }
-            if (score_base != nullptr) {
+            for (uint32_t i = 0; i < kR; ++i) {
+                const bool exists = ((gone >> i) & 1u) == 0u;
+                const uint32_t slot = first + i * kPagedSlice + g;
+                const bool live0 = exists && slot < slots, live1 = exists && slot + 8u < slots;
 #pragma unroll
                 for (uint32_t nt = 0; nt < kTiles; ++nt) {
-                    float* to = score_base + uint64_t(first + g) * (kTiles * 8u) + nt * 8u + 2u * t;
-                    if (first + g < slots) *reinterpret_cast<float2*>(to) = make_float2(x[nt][0], x[nt][1]);
-                    if (first + g + 8u < slots) *reinterpret_cast<float2*>(to + 8u * kTiles * 8u) = make_float2(x[nt][2], x[nt][3]);
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; ++e) {
+                        s[i][nt][e] = (e < 2 ? live0 : live1) ? (s[i][nt][e] + s2[i][nt][e]) * p.scale_log2e : -INFINITY;
+                        higher = higher || s[i][nt][e] > m[nt][e & 1u];
+                    }
+                }
+                if (score_base != nullptr) {
+#pragma unroll
+                    for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                        float* to = score_base + uint64_t(slot) * (kTiles * 8u) + nt * 8u + 2u * t;
+                        if (slot < slots) *reinterpret_cast<float2*>(to) = make_float2(s[i][nt][0], s[i][nt][1]);
+                        if (slot + 8u < slots) *reinterpret_cast<float2*>(to + 8u * kTiles * 8u) = make_float2(s[i][nt][2], s[i][nt][3]);
+                    }
                 }
             }
-            // The maximum rises a few times at the start of an item and hardly ever later: only then is it looked for across the slice's
+            // The maximum rises a few times at the start of an item and hardly ever later: only then is it looked for across the step's
             // slots and everything summed so far scaled down.
             if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
                 for (uint32_t nt = 0; nt < kTiles; ++nt) {
-                    float mx0 = fmaxf(x[nt][0], x[nt][2]), mx1 = fmaxf(x[nt][1], x[nt][3]);
+                    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+                    for (uint32_t i = 0; i < kR; ++i) {
+                        mx0 = fmaxf(mx0, fmaxf(s[i][nt][0], s[i][nt][2]));
+                        mx1 = fmaxf(mx1, fmaxf(s[i][nt][1], s[i][nt][3]));
+                    }
 #pragma unroll
                     for (uint32_t off = 4; off < 32; off <<= 1) {
                         mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, off));
@@ -403,25 +445,32 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                     }
                 }
             }
-            uint32_t pb[kTiles][2];
+            uint32_t pb[kR][kTiles][2];
 #pragma unroll
             for (uint32_t nt = 0; nt < kTiles; ++nt) {
                 const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
-                const float p0 = exp2_fast(x[nt][0] - b0), p1 = exp2_fast(x[nt][1] - b1), p2 = exp2_fast(x[nt][2] - b0), p3 = exp2_fast(x[nt][3] - b1);
-                l[nt][0] += p0 + p2;
-                l[nt][1] += p1 + p3;
-                // the weights are rounded to the cache's type for the second product: half a step each, of random sign
-                pb[nt][0] = movmatrix_trans(Half<T>::pack(p0, p1));   // slots 2t, 2t+1 of head g
-                pb[nt][1] = movmatrix_trans(Half<T>::pack(p2, p3));   // slots 2t+8, 2t+9 of head g
+#pragma unroll
+                for (uint32_t i = 0; i < kR; ++i) {
+                    const float p0 = exp2_fast(s[i][nt][0] - b0), p1 = exp2_fast(s[i][nt][1] - b1);
+                    const float p2 = exp2_fast(s[i][nt][2] - b0), p3 = exp2_fast(s[i][nt][3] - b1);
+                    l[nt][0] += p0 + p2;
+                    l[nt][1] += p1 + p3;
+                    // the weights are rounded to the cache's type for the second product: half a step each, of random sign
+                    pb[i][nt][0] = movmatrix_trans(Half<T>::pack(p0, p1));   // slots 2t, 2t+1 of head g
+                    pb[i][nt][1] = movmatrix_trans(Half<T>::pack(p2, p3));   // slots 2t+8, 2t+9 of head g
+                }
             }
             await_unit();
-            const uint32_t vst = ring + place_out * G::kUnit;
+            const uint32_t vst = ring + place_out * G::kUnit + v_row;
 #pragma unroll
-            for (uint32_t ks = 0; ks < kSteps; ++ks) {
-                uint32_t a0, a1, a2, a3;
-                ldmatrix_x4_trans(vst + v_row + (((ks * 2u + v_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+            for (uint32_t i = 0; i < kR; ++i) {
 #pragma unroll
-                for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                for (uint32_t ks = 0; ks < kSteps; ++ks) {
+                    uint32_t a0, a1, a2, a3;
+                    ldmatrix_x4_trans(vst + i * kPagedSlice * G::kRow + ks / 4u * 128u + (((ks % 4u * 2u + v_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
+#pragma unroll
+                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                }
             }
             release_unit();
         }
