@@ -23,27 +23,31 @@ namespace tb {
 
 constexpr uint32_t kPdWarps = 4, kPdThreads = kPdWarps * 32;
 constexpr float kPdLog2e = 1.4426950408889634f;
-constexpr uint32_t kPdMinPart = 128;          // slots of the shortest partition: two slices for each warp
 constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinDims = 64;
 constexpr uint32_t kJoinPhases = 8;           // the join adds partitions f, f + 8, ... in phase f, then the phases in order
 
 // CTAs of the first kernel that share an SM: their rings fill its shared memory, their accumulators its registers.  Several, so
 // that one streams while another joins its warps, fetches a query or looks up a page.
 __host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim, bool wide) { return head_dim == 256u ? 2u : head_dim == 128u && wide ? 3u : 4u; }
-// The cut of a lane of n slots: partitions of at least 128 slots, and no more items than one CTA for each SM (head_dim 256) or two
+// The cut of a lane of n slots: partitions of at least pd_min_part slots, and no more items than one CTA for each SM (head_dim 256) or two
 // take in one go.  Fewer and longer ones serve a batch better (fewer records), more of them would only help a lane alone.
 __host__ __device__ inline uint32_t pd_per_wave(uint32_t kv_heads, uint32_t head_dim) {
     const uint32_t p = kSmCount * (head_dim == 256u ? 1u : 2u) / kv_heads;
     return p == 0u ? 1u : p;
 }
-__host__ __device__ inline uint32_t pd_part_slots(uint32_t n, uint32_t per_wave) {
-    if (n <= per_wave * kPdMinPart) return kPdMinPart;
-    return ((n + per_wave - 1u) / per_wave + kPagedSlice - 1u) / kPagedSlice * kPagedSlice;
-}
-__host__ __device__ inline uint32_t pd_parts(uint32_t n, uint32_t per_wave) {
-    const uint32_t p = pd_part_slots(n, per_wave);
-    return (n + p - 1u) / p;
-}
+// Slots of the shortest partition: its records (head_dim x group floats) stay below a sixteenth of its rows.
+__host__ __device__ inline uint32_t pd_min_part(uint32_t group) { return group <= 8u ? 128u : 256u; }
+struct PagedCut {
+    uint32_t per_wave, least;
+    __host__ __device__ uint32_t part_slots(uint32_t n) const {
+        if (n <= per_wave * least) return least;
+        return ((n + per_wave - 1u) / per_wave + kPagedSlice - 1u) / kPagedSlice * kPagedSlice;
+    }
+    __host__ __device__ uint32_t parts(uint32_t n) const {
+        const uint32_t s = part_slots(n);
+        return (n + s - 1u) / s;
+    }
+};
 
 struct PagedDecodeParams {
     PagedView cache;
@@ -55,7 +59,8 @@ struct PagedDecodeParams {
     float2* stats;     // [lane][q head][part]: maximum (log2 units), sum
     float* scores;     // [lane][kv head][max_keys rounded up to 16][group rounded up to 8], log2 units; null without a mass
     uint64_t query_stride;
-    uint32_t n_lanes, max_keys, q_heads, group, per_wave;
+    uint32_t n_lanes, max_keys, q_heads, group;
+    PagedCut cut;
     uint32_t parts;        // parts of the longest lane: the stride of sums and stats
     uint32_t score_slots;  // max_keys rounded up to 16
     uint32_t units;        // places of a warp's ring
@@ -197,13 +202,13 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     const uint64_t policy = l2_evict_first_policy();
     wait_for_predecessor();
     release_dependents();
-    scan_items<kPdThreads>(p, item_start, lane_keys, warp_word, blockIdx.x == 0, [&](uint32_t n) { return pd_parts(n, p.per_wave); });
+    scan_items<kPdThreads>(p, item_start, lane_keys, warp_word, blockIdx.x == 0, [&](uint32_t n) { return p.cut.parts(n); });
     const uint32_t total = item_start[p.n_lanes];
     // this CTA's items are blockIdx.x, blockIdx.x + gridDim.x, ...; a thread describes one
     const uint32_t count = total > blockIdx.x ? (total - 1u - blockIdx.x) / gridDim.x + 1u : 0u;
     auto describe = [&](uint32_t k) {
         if (k >= count) return;
-        const PagedItem it = item_at(p, item_start, lane_keys, blockIdx.x + k * gridDim.x, [&](uint32_t n) { return pd_part_slots(n, p.per_wave); });
+        const PagedItem it = item_at(p, item_start, lane_keys, blockIdx.x + k * gridDim.x, [&](uint32_t n) { return p.cut.part_slots(n); });
         items[k % kPdItems] = make_uint4(it.lane | it.kv << 16, it.part, it.begin, it.slots);
     };
     describe(threadIdx.x);
@@ -554,7 +559,9 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 // head each.
 constexpr uint32_t kMassSpan = 1024;
 
-template <typename T, int D>
+// A piece is finished by the CTA, or by one warp where no lane has more than 16 partitions: the same additions in the same order, so
+// the form is free to follow from max_keys.
+template <typename T, int D, bool kByWarp>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t walkers) {
     __shared__ uint32_t item_start[TATARA_MAX_LANES + 1], lane_keys[TATARA_MAX_LANES], warp_total[kJoinWarps];
@@ -567,19 +574,69 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
     wait_for_predecessor();
     release_dependents();
     if (blockIdx.x >= walkers) {
-        const uint32_t piece = blockIdx.x - walkers, slice = piece % kSlices, rest = piece / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
+        const uint32_t piece = kByWarp ? (blockIdx.x - walkers) * kJoinWarps + warp : blockIdx.x - walkers;
+        const uint32_t slice = piece % kSlices, rest = piece / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
+        if (row >= p.n_lanes) return;
         const uint32_t n = __ldcg(&p.lanes[row].keys);
         if (n > p.max_keys) return;                        // refused: its row stays as it is
-        const uint32_t parts = n == 0u ? 0u : pd_parts(n, p.per_wave);
+        const uint32_t parts = n == 0u ? 0u : p.cut.parts(n);
         const uint64_t record = (uint64_t(row) * p.q_heads + head) * p.parts;
-        const uint32_t pair = threadIdx.x & 31u, phase = threadIdx.x >> 5;
-        const uint64_t at = (row * p.query_stride + uint64_t(head) * D + slice * kJoinDims + threadIdx.x) * 2u;
+        const uint32_t pair = lane, phase = warp;
+        const float* base = p.sums + record * D + slice * kJoinDims + pair * 2u;
+        const uint64_t out_row = row * p.query_stride + uint64_t(head) * D + slice * kJoinDims;
+        if constexpr (kByWarp) {
+            const uint64_t at = (out_row + pair * 2u) * 2u;
+            float gate0 = 0.0f, gate1 = 0.0f;
+            if (p.gate != nullptr) {
+                gate0 = Half<T>::load(p.gate + at);
+                gate1 = Half<T>::load(p.gate + at + 2u);
+            }
+            const float2 ml = lane < parts ? __ldcg(&p.stats[record + lane]) : make_float2(-INFINITY, 0.0f);
+            float a[kJoinPhases][2];
+#pragma unroll
+            for (uint32_t f = 0; f < kJoinPhases; ++f) a[f][0] = a[f][1] = 0.0f;
+            float top = ml.x, mine = 0.0f, sum = 0.0f;
+#pragma unroll
+            for (uint32_t off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            mine = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
+            sum = fmaf(mine, ml.y, 0.0f);
+#pragma unroll
+            for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+            for (uint32_t part0 = 0; part0 < parts; part0 += kJoinPhases) {
+                float2 x[kJoinPhases];
+#pragma unroll
+                for (uint32_t f = 0; f < kJoinPhases; ++f)
+                    if (part0 + f < parts) x[f] = __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part0 + f) * D));
+#pragma unroll
+                for (uint32_t f = 0; f < kJoinPhases; ++f) {
+                    const float w = __shfl_sync(0xffffffffu, mine, (part0 + f) & 31u);
+                    if (part0 + f < parts) {
+                        a[f][0] = fmaf(w, x[f].x, a[f][0]);
+                        a[f][1] = fmaf(w, x[f].y, a[f][1]);
+                    }
+                }
+            }
+            float n0 = 0.0f, n1 = 0.0f;
+#pragma unroll
+            for (uint32_t f = 0; f < kJoinPhases; ++f) {
+                n0 += a[f][0];
+                n1 += a[f][1];
+            }
+            float r0 = sum == 0.0f ? 0.0f : n0 / sum, r1 = sum == 0.0f ? 0.0f : n1 / sum;   // no slot at all: zero
+            if (p.gate != nullptr) {
+                r0 *= 1.0f / (1.0f + expf(-gate0));
+                r1 *= 1.0f / (1.0f + expf(-gate1));
+            }
+            Half<T>::store(p.out + at, r0);
+            Half<T>::store(p.out + at + 2u, r1);
+            return;
+        }
+        const uint64_t at = (out_row + threadIdx.x) * 2u;
         float gate = 0.0f;
         if (threadIdx.x < kJoinDims && p.gate != nullptr) gate = Half<T>::load(p.gate + at);
         // the first partitions' sums are asked for before their weights are known
         constexpr uint32_t kAhead = 10;
         float2 v[kAhead];
-        const float* base = p.sums + record * D + slice * kJoinDims + pair * 2u;
 #pragma unroll
         for (uint32_t i = 0; i < kAhead; ++i) {
             const uint32_t part = phase + i * kJoinPhases;
@@ -638,7 +695,7 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
     const uint32_t total = item_start[p.n_lanes], row_floats = (p.group + 7u) / 8u * 8u;
     for (uint32_t item = blockIdx.x; item < total; item += walkers) {
         const PagedItem it = item_at(p, item_start, lane_keys, item, [](uint32_t) { return kMassSpan; });
-        const uint32_t parts = pd_parts(lane_keys[it.lane], p.per_wave);
+        const uint32_t parts = p.cut.parts(lane_keys[it.lane]);
         const uint64_t head_row = uint64_t(it.lane) * p.cache.kv_heads + it.kv;
         const float* scores = p.scores + (head_row * p.score_slots + it.begin) * row_floats;
         float* mass = p.cache.mass + head_row * p.cache.capacity + it.begin;
@@ -702,14 +759,15 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
 
 // ---- host side -------------------------------------------------------------------------
 struct PagedDecodeLayout {
-    uint32_t per_wave, parts, score_slots, row_floats;
+    PagedCut cut;
+    uint32_t parts, score_slots, row_floats;
     uint64_t stats_at, scores_at, bytes;
 };
 static PagedDecodeLayout pd_layout(const tatara_paged_cache& c, uint32_t n_lanes, uint32_t max_keys, uint32_t q_heads) {
     PagedDecodeLayout l{};
-    l.per_wave = pd_per_wave(c.kv_heads, c.head_dim);
-    const uint32_t shortest = (max_keys + kPdMinPart - 1u) / kPdMinPart;   // pd_parts(n) <= both for every n <= max_keys
-    l.parts = shortest < l.per_wave ? shortest : l.per_wave;
+    l.cut = PagedCut{pd_per_wave(c.kv_heads, c.head_dim), pd_min_part(q_heads / c.kv_heads)};
+    const uint32_t shortest = (max_keys + l.cut.least - 1u) / l.cut.least;   // cut.parts(n) <= both for every n <= max_keys
+    l.parts = shortest < l.cut.per_wave ? shortest : l.cut.per_wave;
     l.score_slots = (max_keys + kPagedSlice - 1u) / kPagedSlice * kPagedSlice;
     l.row_floats = (q_heads / c.kv_heads + 7u) / 8u * 8u;
     const uint64_t records = uint64_t(n_lanes) * q_heads * l.parts;
@@ -738,7 +796,10 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
     const uint64_t spans = uint64_t(p.n_lanes) * p.cache.kv_heads * ((p.max_keys + kMassSpan - 1u) / kMassSpan);
     const uint32_t walkers = p.cache.mass == nullptr ? 0u : uint32_t(spans < 4u * ctx->sm_count ? spans : 4u * ctx->sm_count);
-    (void)launch_staged(paged_join_kernel<T, D>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
+    if (p.parts <= 16u)
+        (void)launch_staged(paged_join_kernel<T, D, true>, dim3((pieces + kJoinWarps - 1u) / kJoinWarps + walkers), kJoinThreads, 0u, stream, p, walkers);
+    else
+        (void)launch_staged(paged_join_kernel<T, D, false>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
     return check_launch(ctx, "attn_decode_paged: join");
 }
 
@@ -795,7 +856,7 @@ extern "C" tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream,
     p.max_keys = max_keys;
     p.q_heads = q_heads;
     p.group = q_heads / cache->kv_heads;
-    p.per_wave = l.per_wave;
+    p.cut = l.cut;
     p.parts = l.parts;
     p.score_slots = l.score_slots;
     p.page_slices = cache->page_slots / kPagedSlice;

@@ -20,7 +20,7 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t kSelThreads = 1024, kSelWarps = kSelThreads / 32, kSelBins = 2048, kSelMaxCluster = 16, kSelMaxKeys = 16;
 static_assert(kSelThreads * kSelMaxKeys * kSelMaxCluster >= TATARA_MAX_CONTEXT, "one cluster holds the longest lane");
-constexpr uint32_t kMoveThreads = 256, kMoveBatch = 4;
+constexpr uint32_t kMoveThreads = 256, kMoveBatch = 2;
 
 struct PagedEvictParams {
     PagedView cache;
@@ -312,8 +312,8 @@ paged_move_kernel(const __grid_constant__ PagedEvictParams p) {
 #pragma unroll
         for (uint32_t i = 0; i < kMoveBatch; ++i) {
             if (live[i]) {
-                *reinterpret_cast<uint4*>(p.cache.keys + to[i]) = k[i];
-                *reinterpret_cast<uint4*>(p.cache.values + to[i]) = v[i];
+                __stcs(reinterpret_cast<uint4*>(p.cache.keys + to[i]), k[i]);
+                __stcs(reinterpret_cast<uint4*>(p.cache.values + to[i]), v[i]);
             }
         }
     }
