@@ -167,7 +167,8 @@ struct PdGeometry {
     static constexpr uint32_t kSlices = D == 64 ? 2 : 1, kStep = kSlices * kPagedSlice;
     static constexpr uint32_t kRow = D * 2, kChunks = D / 8, kUnit = kStep * kRow;
     static constexpr uint32_t kMaxUnits = 6;
-    static constexpr uint32_t smem(uint32_t units) { return kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
+    static constexpr uint32_t query(bool wide) { return wide ? 16u * kRow : 0u; }   // sixteen heads do not fit in registers beside their sums
+    static constexpr uint32_t smem(uint32_t units, bool wide) { return query(wide) + kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
     // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and the rest of the SM's memory
     // serves the copies better as L1 than as a deeper ring.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings an SM, 93 - 99 at
     // 160 to 192; 32 lanes of 16384: 189 us at 128 KiB, 205 at 192.
@@ -193,7 +194,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     constexpr uint32_t kSteps = D / 16, kR = G::kSlices, kStep = G::kStep;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u;
-    uint4* items = reinterpret_cast<uint4*>(smem + kPdWarps * p.units * G::kUnit);    // {lane | kv << 16, part, begin, slots}
+    uint8_t* query = smem + kPdWarps * p.units * G::kUnit;
+    uint4* items = reinterpret_cast<uint4*>(query + G::query(kTiles == 2));    // {lane | kv << 16, part, begin, slots}
     float2* merge_ml = reinterpret_cast<float2*>(items + kPdItems);
     uint32_t* item_start = reinterpret_cast<uint32_t*>(merge_ml + kPdWarps * 8);
     uint32_t* lane_keys = item_start + TATARA_MAX_LANES + 1;
@@ -338,22 +340,44 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     const uint32_t k_row = ((lm_j & 1u) * 8u + lm_r) * G::kRow, k_chunk = lm_j >> 1;
     const uint32_t v_row = ((lm_j >> 1) * 8u + lm_r) * G::kRow, v_chunk = lm_j & 1u;
 
-    uint32_t qf[kTiles][kSteps][2];
+    // Q as the B operand: of up to eight heads in registers, lane (g, t) holding dims 16 ks + 2t, +1 | +8, +9 of head g; of more, out of
+    // shared memory step by step (rows swizzled as the units are).
+    uint32_t qf[kTiles == 1 ? kSteps : 1][2];
+    uint4 qn[kTiles == 2 ? D / 64 : 1];
+    const uint32_t q_row = smem_u32(query) + ((lm_j >> 1) * 8u + lm_r) * G::kRow, q_chunk = lm_j & 1u;
     auto load_query = [&](const uint4& it) {
-#pragma unroll
-        for (uint32_t nt = 0; nt < kTiles; ++nt) {
-            const uint32_t head = nt * 8u + g;
-            const uint32_t* row = reinterpret_cast<const uint32_t*>(
-                p.q + ((it.x & 0xFFFFu) * p.query_stride + uint64_t((it.x >> 16) * p.group + (head < p.group ? head : 0u)) * D) * 2u);
+        const uint8_t* base = p.q + ((it.x & 0xFFFFu) * p.query_stride + uint64_t((it.x >> 16) * p.group) * D) * 2u;
+        if constexpr (kTiles == 1) {
+            const uint32_t* row = reinterpret_cast<const uint32_t*>(base + (g < p.group ? g : 0u) * (D * 2u));
 #pragma unroll
             for (uint32_t ks = 0; ks < kSteps; ++ks) {
-                qf[nt][ks][0] = head < p.group ? __ldcg(row + ks * 8u + t) : 0u;
-                qf[nt][ks][1] = head < p.group ? __ldcg(row + ks * 8u + 4u + t) : 0u;
+                qf[ks][0] = g < p.group ? __ldcg(row + ks * 8u + t) : 0u;
+                qf[ks][1] = g < p.group ? __ldcg(row + ks * 8u + 4u + t) : 0u;
+            }
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < D / 64; ++i) {
+                const uint32_t c = threadIdx.x + i * kPdThreads, head = c / G::kChunks;
+                const uint32_t* from = reinterpret_cast<const uint32_t*>(base + (head < p.group ? c : 0u) * 16u);
+                qn[i] = head < p.group ? make_uint4(__ldcg(from), __ldcg(from + 1), __ldcg(from + 2), __ldcg(from + 3)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        }
+    };
+    auto store_query = [&]() {
+        if constexpr (kTiles == 2) {
+#pragma unroll
+            for (uint32_t i = 0; i < D / 64; ++i) {
+                const uint32_t c = threadIdx.x + i * kPdThreads, head = c / G::kChunks;
+                *reinterpret_cast<uint4*>(query + head * G::kRow + (((c % G::kChunks) ^ (head & 7u)) << 4)) = qn[i];
             }
         }
     };
     uint4 ci = pi;
-    if (count != 0u) load_query(ci);
+    if (count != 0u) {
+        load_query(ci);
+        store_query();
+    }
+    if constexpr (kTiles == 2) __syncthreads();
     while (done_items < count) {
         float o[kTiles][kSteps][4], m[kTiles][2], l[kTiles][2];
 #pragma unroll
@@ -380,15 +404,19 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 #pragma unroll
                     for (uint32_t e = 0; e < 4; ++e) s[i][nt][e] = s2[i][nt][e] = 0.0f;
 #pragma unroll
-                for (uint32_t ks = 0; ks < kSteps; ks += 2) {
+                for (uint32_t ks = 0; ks < kSteps; ++ks) {
                     uint32_t a0, a1, a2, a3;
                     // (the swizzle only touches the low three bits of a chunk: every fourth step shares its offset)
                     ldmatrix_x4(kst + i * kPagedSlice * G::kRow + ks / 4u * 128u + (((ks % 4u * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
-#pragma unroll
-                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s[i][nt], a0, a1, a2, a3, qf[nt][ks][0], qf[nt][ks][1]);
-                    ldmatrix_x4(kst + i * kPagedSlice * G::kRow + ks / 4u * 128u + ((((ks + 1u) % 4u * 2u + k_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
-#pragma unroll
-                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(s2[i][nt], a0, a1, a2, a3, qf[nt][ks + 1][0], qf[nt][ks + 1][1]);
+                    float (&sum)[kTiles][4] = ks % 2u == 0u ? s[i] : s2[i];   // two chains of additions
+                    if constexpr (kTiles == 1) {
+                        Half<T>::mma(sum[0], a0, a1, a2, a3, qf[ks][0], qf[ks][1]);
+                    } else {
+                        uint32_t b0, b1, b2, b3;
+                        ldmatrix_x4(q_row + ks / 4u * 128u + (((ks % 4u * 2u + q_chunk) ^ lm_r) << 4), b0, b1, b2, b3);
+                        Half<T>::mma(sum[0], a0, a1, a2, a3, b0, b1);
+                        Half<T>::mma(sum[kTiles - 1], a0, a1, a2, a3, b2, b3);
+                    }
                 }
             }
             release_unit();
@@ -545,6 +573,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                 }
                 if ((threadIdx.x & 15u) == 0u) p.stats[record] = make_float2(top, sum);
             }
+            // every warp has read this item's query: the next one's takes its place
+            if (nt == 0u) store_query();
             // half of the descriptors lie behind every warp: the half after the other one takes their place
             if (nt + 1u == kTiles && done_items % (kPdItems / 2u) == 0u && threadIdx.x < kPdItems / 2u)
                 describe(done_items + kPdItems / 2u + threadIdx.x);
@@ -783,14 +813,14 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     constexpr uint32_t kCtas = pd_ctas(D, kTiles == 2);
     static bool configured[64] = {false};
     if (!configured[ctx->device & 63]) {
-        if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(G::units(1u))) != cudaSuccess)
+        if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(G::units(1u), kTiles == 2)) != cudaSuccess)
             return check_launch(ctx, "attn_decode_paged: shared memory attribute");
         configured[ctx->device & 63] = true;
     }
     const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, sms = ctx->sm_count;
     const uint32_t ctas = items >= kCtas * sms ? kCtas : uint32_t((items + sms - 1u) / sms);   // on an SM
     p.units = G::units(ctas);
-    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < kCtas * sms ? items : kCtas * sms)), kPdThreads, G::smem(p.units), stream, p);
+    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < kCtas * sms ? items : kCtas * sms)), kPdThreads, G::smem(p.units, kTiles == 2), stream, p);
     const tatara_status st = check_launch(ctx, "attn_decode_paged");
     if (st != TATARA_OK) return st;
     const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
