@@ -96,8 +96,8 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 
 // ---- q/k norm + rope + append --------------------------------------------------------------
 // A warp owns one (head, row): lane l holds dims 8l .. 8l+7 (16-byte accesses), dims d and d + 32 of a rotated pair are
-// four lanes apart.  A lane evaluates the angles of the eight pairs that its own dims need, in turns: the product and
-// the fraction in double, since a far position loses its angle in f32 (2^18 / 1.6 has a last place of 1/64), then one sincospif.
+// four lanes apart.  Lane l evaluates the angle of pair l, in turns: the product and the fraction in double, since a far position
+// loses its angle in f32 (2^18 / 1.6 has a last place of 1/64), then one sincospif; lanes 0 .. 7 take theirs by shuffles.
 constexpr uint32_t kRopeWarps = 4;
 
 struct PagedRopeParams {
@@ -128,19 +128,20 @@ paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     const uint32_t row = unit / (kQHeads + kKvHeads), head = unit - row * (kQHeads + kKvHeads);
     if (row >= p.n_lanes) return;
     wait_for_predecessor();
-    const uint2 l = __ldcg(reinterpret_cast<const uint2*>(p.lanes + row));   // keys, position
-    if (l.x == 0u) return;                                                   // idle
     const bool is_q = head < kQHeads;
     const uint32_t local = is_q ? head : head - kQHeads;
-    if (l.x > p.cache.capacity) {
-        if (lane == 0) latch_out_of_range(p.cache, row);
-        return;
-    }
     const __nv_bfloat16* proj = p.projection + row * p.projection_stride;
+    // (every load is on its way before the lane's state decides; an idle lane has a projection row too)
+    const uint2 l = __ldcg(reinterpret_cast<const uint2*>(p.lanes + row));   // keys, position
     const uint4 raw = __ldcg(reinterpret_cast<const uint4*>(proj + (is_q ? head * 2u * kHeadDim : kAttnKOff + local * kHeadDim) + lane * 8u));
     // what is copied through: the gate of a query head, the values of a key head
     const uint4 through = __ldcg(reinterpret_cast<const uint4*>(proj + (is_q ? head * 2u * kHeadDim + kHeadDim : kAttnVOff + local * kHeadDim) + lane * 8u));
     const uint4 wraw = __ldcg(reinterpret_cast<const uint4*>((is_q ? p.q_weight : p.k_weight) + lane * 8u));
+    if (l.x == 0u) return;                                                   // idle
+    if (l.x > p.cache.capacity) {
+        if (lane == 0) latch_out_of_range(p.cache, row);
+        return;
+    }
     float x[8], w[8];
     unpack8(raw, x);
     unpack8(wraw, w);
@@ -149,17 +150,17 @@ paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     for (uint32_t i = 0; i < 8; ++i) acc = fmaf(x[i], x[i], acc);
     acc = warp_sum(acc);
     const float inverse = 1.0f / sqrtf(acc / float(kHeadDim) + kRmsEps);
+    const double turns = double(l.y) * p.turns[lane];
+    float sine, cosine;
+    sincospif(2.0f * float(turns - rint(turns)), &sine, &cosine);
     __nv_bfloat16 res[8];
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         x[i] = w[i] * (x[i] * inverse);
+        const uint32_t pair = (lane & 3u) * 8u + i;
         const float partner = __shfl_xor_sync(0xffffffffu, x[i], 4);   // dim +- 32 (used by lanes 0..7)
-        if (lane < 8u) {
-            const double turns = double(l.y) * p.turns[(lane & 3u) * 8u + i];
-            float sine, cosine;
-            sincospif(2.0f * float(turns - rint(turns)), &sine, &cosine);
-            x[i] = lane < 4u ? fmaf(-partner, sine, x[i] * cosine) : fmaf(partner, sine, x[i] * cosine);
-        }
+        const float s = __shfl_sync(0xffffffffu, sine, pair), c = __shfl_sync(0xffffffffu, cosine, pair);
+        if (lane < 8u) x[i] = lane < 4u ? fmaf(-partner, s, x[i] * c) : fmaf(partner, s, x[i] * c);
         res[i] = f2bf(x[i]);
     }
     if (is_q) {
@@ -182,9 +183,10 @@ paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
 // ---- the lane table between tokens ---------------------------------------------------------
 __global__ void paged_lanes_step_kernel(tatara_paged_lane* lanes, uint32_t n_lanes, uint32_t keep, uint32_t advance) {
     const uint32_t i = threadIdx.x;
-    if (i >= n_lanes || lanes[i].keys == 0u) return;
-    lanes[i].keys = min(lanes[i].keys, keep) + advance;
-    lanes[i].position += advance;
+    wait_for_predecessor();
+    if (i >= n_lanes) return;
+    const uint2 l = __ldcg(reinterpret_cast<const uint2*>(lanes + i));   // keys, position
+    if (l.x != 0u) lanes[i] = tatara_paged_lane{min(l.x, keep) + advance, l.y + advance};
 }
 
 } // namespace tb
@@ -267,6 +269,6 @@ extern "C" tatara_status tatara_paged_lanes_step(tatara_ctx* ctx, void* stream, 
     if (n_lanes == 0 || n_lanes > TATARA_MAX_LANES) return fail(ctx, TATARA_INVALID_STREAM_GROUP, "paged_lanes_step: lane count");
     if (keep == 0 || advance > TATARA_MAX_CONTEXT) return fail(ctx, TATARA_INVALID_DISPATCH_EXTENT, "paged_lanes_step: keep, advance");
     const DeviceGuard guard(ctx);
-    paged_lanes_step_kernel<<<1, TATARA_MAX_LANES, 0, static_cast<cudaStream_t>(stream)>>>(lanes_device, n_lanes, keep, advance);
+    (void)launch_staged(paged_lanes_step_kernel, dim3(1), TATARA_MAX_LANES, 0u, static_cast<cudaStream_t>(stream), lanes_device, n_lanes, keep, advance);
     return check_launch(ctx, "paged_lanes_step");
 }

@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t walkers) {
     __shared__ uint32_t item_start[TATARA_MAX_LANES + 1], lane_keys[TATARA_MAX_LANES], warp_total[kJoinWarps];
     __shared__ float weight[kSmCount * 2];                 // per_wave at most
-    __shared__ float red[kJoinWarps];
+    __shared__ float red[kJoinWarps], red_sum[kJoinWarps];
     __shared__ __align__(16) float acc_s[kJoinPhases][kJoinDims];
     __shared__ float2 final_ml[16];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -672,8 +672,14 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
             const uint32_t part = phase + i * kJoinPhases;
             v[i] = part < parts ? __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D)) : make_float2(0.0f, 0.0f);
         }
-        float top = -INFINITY;
-        for (uint32_t part = threadIdx.x; part < parts; part += kJoinThreads) top = fmaxf(top, __ldcg(&p.stats[record + part]).x);
+        static_assert(kSmCount * 2u <= 2u * kJoinThreads, "two partitions a thread");
+        float2 ml[2];
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t part = threadIdx.x + i * kJoinThreads;
+            ml[i] = part < parts ? __ldcg(&p.stats[record + part]) : make_float2(-INFINITY, 0.0f);
+        }
+        float top = fmaxf(ml[0].x, ml[1].x);
 #pragma unroll
         for (uint32_t off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
         if (lane == 0) red[warp] = top;
@@ -681,17 +687,17 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
         top = red[0];
 #pragma unroll
         for (uint32_t w = 1; w < kJoinWarps; ++w) top = fmaxf(top, red[w]);
-        __syncthreads();
         float sum = 0.0f;
-        for (uint32_t part = threadIdx.x; part < parts; part += kJoinThreads) {
-            const float2 ml = __ldcg(&p.stats[record + part]);
-            const float w = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - top);
-            weight[part] = w;
-            sum = fmaf(w, ml.y, sum);
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t part = threadIdx.x + i * kJoinThreads;
+            const float w = ml[i].x == -INFINITY ? 0.0f : exp2f(ml[i].x - top);
+            if (part < parts) weight[part] = w;
+            sum = fmaf(w, ml[i].y, sum);
         }
 #pragma unroll
         for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (lane == 0) red[warp] = sum;
+        if (lane == 0) red_sum[warp] = sum;
         __syncthreads();
         float a0 = 0.0f, a1 = 0.0f;
 #pragma unroll
@@ -714,7 +720,7 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
 #pragma unroll
             for (uint32_t ph = 0; ph < kJoinPhases; ++ph) num += acc_s[ph][threadIdx.x];
 #pragma unroll
-            for (uint32_t w = 0; w < kJoinWarps; ++w) den += red[w];
+            for (uint32_t w = 0; w < kJoinWarps; ++w) den += red_sum[w];
             float r = den == 0.0f ? 0.0f : num / den;      // no slot at all: zero
             if (p.gate != nullptr) r *= 1.0f / (1.0f + expf(-gate));
             Half<T>::store(p.out + at, r);
