@@ -372,8 +372,9 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
             }
         }
     };
-    uint4 ci = pi;
+    uint4 ci = make_uint4(0u, 0u, 0u, 0u);
     if (count != 0u) {
+        ci = items[0];      // (a warp that has no share of the first items reads ahead of them already)
         load_query(ci);
         store_query();
     }

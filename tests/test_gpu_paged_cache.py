@@ -87,6 +87,22 @@ def test_long_lanes_and_many_heads(ctx, kv_heads, group, dim, n, page):
     assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
 
 
+@pytest.mark.parametrize("kv_heads,group,dim,most", [(2, 8, 256, 300), (3, 16, 256, 40), (8, 4, 128, 200), (4, 11, 128, 17), (12, 1, 64, 70),
+                                                     (16, 16, 64, 300), (64, 2, 64, 20)])
+def test_many_short_lanes(ctx, kv_heads, group, dim, most):
+    """Far more partitions than CTAs, most of them too short for every warp to have a share, of lanes in any mixture of lengths."""
+    rng = np.random.default_rng(most)
+    lens = [int(x) for x in rng.integers(0, most + 1, 256)]
+    lens[100], lens[101] = 3 * most + 400, 1
+    c = Cache(lens, kv_heads, dim, page=32, seed=most)
+    q, gate = query(c, kv_heads * group)
+    want, bound, added, added_bound = decode_definition(c, q, gate, dim ** -0.5)
+    before = c.mass.double()
+    out = decode(ctx, c, q, gate)
+    assert ((out.double() - want).abs() <= bound).all()
+    assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
+
+
 def test_the_longest_context(ctx):
     c = Cache([262144], 2, 256, page=64, seed=9, extra_columns=0)
     q, gate = query(c, 16)
