@@ -172,7 +172,9 @@ def paged_cache(keys, values, page_table, mass=None, positions=None) -> PagedCac
             raise ValueError(f"paged_cache: {name} is {list(plane)} {dtype}, contiguous")
     if any(t is not None and t.device != keys.device for t in (values, page_table, mass, positions)):
         raise ValueError("paged_cache: tensors on one device")
-    c = PagedCache(keys.data_ptr(), values.data_ptr(), keys.stride(0), keys.stride(1), keys.stride(2),
+    # (a dimension of one has no stride that means anything)
+    page_stride, head_stride, slot_stride = (s if n > 1 else dim for s, n in zip(keys.stride(), keys.shape[:3]))
+    c = PagedCache(keys.data_ptr(), values.data_ptr(), page_stride, head_stride, slot_stride,
                    page_table.data_ptr(), None if mass is None else mass.data_ptr(), None if positions is None else positions.data_ptr(),
                    page_table.shape[0], page_table.shape[1], pages, slots, heads, dim, kinds[keys.dtype], 0)
     c.tensors = (keys, values, page_table, mass, positions)
@@ -437,6 +439,12 @@ class Context:
                 return t.stride(0)
         raise ValueError(f"{what}: at least {n} rows of {row} contiguous elements in the cache's type, on its device")
 
+    @staticmethod
+    def _paged_scratch(scratch, cache):
+        if scratch.get_device() != cache.device or not scratch.is_contiguous():
+            raise ValueError("scratch: contiguous, on the cache's device")
+        return scratch.data_ptr(), scratch.numel() * scratch.element_size()
+
     def _paged_lanes(self, lanes, cache=None):
         _bind_torch()
         shape = lanes.shape
@@ -453,8 +461,9 @@ class Context:
                 values.stride() != strides or keys.dtype is not cache.torch_dtype or values.dtype is not cache.torch_dtype or keys.get_device() != cache.device or \
                 values.get_device() != cache.device:
             raise ValueError("paged_append: keys and values are alike, [row][kv head][dim] in the cache's type")
-        if row_starts is not None and (row_starts.dtype is not _torch.int32 or row_starts.numel() != n + 1 or not row_starts.is_contiguous()):
-            raise ValueError("paged_append: row_starts is int32 [lanes + 1]")
+        if row_starts is not None and (row_starts.dtype is not _torch.int32 or row_starts.numel() != n + 1 or not row_starts.is_contiguous() or
+                                       row_starts.get_device() != cache.device):
+            raise ValueError("paged_append: row_starts is int32 [lanes + 1], contiguous, on the cache's device")
         # (a dimension of one has no stride that means anything)
         self._check(lib().tatara_paged_append(
             self._h, self._paged_stream(stream), cache.ref, at, n, keys.data_ptr(), values.data_ptr(),
@@ -467,6 +476,9 @@ class Context:
         stride = self._paged_rows("attn_qk_rope_paged: q_out", q_out, cache, n, Q_HEADS * HEAD_DIM)
         if self._paged_rows("attn_qk_rope_paged: gate_out", gate_out, cache, n, Q_HEADS * HEAD_DIM) != stride:
             raise ValueError("attn_qk_rope_paged: q_out and gate_out have one stride")
+        for w in (q_weight, k_weight):
+            if w.dtype is not cache.torch_dtype or w.numel() != HEAD_DIM or w.get_device() != cache.device or not w.is_contiguous():
+                raise ValueError(f"attn_qk_rope_paged: weights of {HEAD_DIM} contiguous elements in the cache's type, on its device")
         self._check(lib().tatara_attn_qk_rope_paged(
             self._h, self._paged_stream(stream), cache.ref, at, n, projection.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(),
             q_out.data_ptr(), gate_out.data_ptr(), self._paged_rows("attn_qk_rope_paged: projection", projection, cache, n, ATTN_PROJ), stride))
@@ -480,17 +492,19 @@ class Context:
         if self._paged_rows("attn_decode_paged: out", out, cache, n, q_heads * dim) != stride or \
                 gate is not None and self._paged_rows("attn_decode_paged: gate", gate, cache, n, q_heads * dim) != stride:
             raise ValueError("attn_decode_paged: q, gate and out have one stride")
+        scratch_at, scratch_bytes = self._paged_scratch(scratch, cache)
         self._check(lib().tatara_attn_decode_paged(
             self._h, self._paged_stream(stream), cache.ref, at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
             q.data_ptr(), None if gate is None else gate.data_ptr(), q_heads, stride, dim ** -0.5 if scale is None else scale,
-            out.data_ptr(), scratch.data_ptr(), scratch.numel() * scratch.element_size()))
+            out.data_ptr(), scratch_at, scratch_bytes))
 
     def paged_evict(self, cache, lanes, keep, scratch, sink=0, recent=0, max_keys=None, stream=None):
         """Trims every lane to at most `keep` slots; paged_lanes_step(lanes, keep=keep) then cuts the lane table."""
         at, n = self._paged_lanes(lanes, cache)
+        scratch_at, scratch_bytes = self._paged_scratch(scratch, cache)
         self._check(lib().tatara_paged_evict(
             self._h, self._paged_stream(stream), cache.ref, at, n, min(cache.capacity, MAX_CONTEXT) if max_keys is None else max_keys,
-            keep, sink, recent, scratch.data_ptr(), scratch.numel() * scratch.element_size()))
+            keep, sink, recent, scratch_at, scratch_bytes))
 
     def paged_lanes_step(self, lanes, keep=NO_CUT, advance=1, stream=None):
         at, n = self._paged_lanes(lanes)

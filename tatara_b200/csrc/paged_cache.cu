@@ -217,7 +217,9 @@ extern "C" tatara_status tatara_paged_append(tatara_ctx* ctx, void* stream, cons
     p.row_starts = row_starts;
     p.n_lanes = n_lanes;
     p.n_rows = n_rows;
-    p.tile_rows = 16u;
+    // rows of a CTA: one while there are SMs to spare, up to 16 to share the look-ups
+    const uint32_t spread = n_rows / (2u * uint32_t(ctx->sm_count));
+    p.tile_rows = spread < 1u ? 1u : spread > 16u ? 16u : spread;
     const uint32_t tiles = (n_rows + p.tile_rows - 1u) / p.tile_rows;
     const DeviceGuard guard(ctx);
     auto kernel = cache->head_dim == 64u ? paged_append_kernel<8> : cache->head_dim == 128u ? paged_append_kernel<16> : paged_append_kernel<32>;

@@ -1,5 +1,6 @@
 """Paged KV cache operators on the device, against their 64-bit definitions (tests/paged_util.py)."""
 import os
+import subprocess
 import sys
 
 import numpy as np
@@ -158,6 +159,31 @@ def test_strided_rows_of_queries_and_outputs(ctx):
     ctx.sync()
     assert ((out.double() - want).abs() <= bound).all()
     assert same(wide[2][:, :10], edge[2][:, :10]) and same(wide[2][:, 1034:], edge[2][:, 1034:]) and same(wide[:2], edge[:2])
+
+
+@pytest.mark.parametrize("kv_heads", [1, 3])
+def test_pools_inside_one_allocation(ctx, kv_heads):
+    """K and V side by side in one tensor, pages with a gap behind them: every stride its own."""
+    lens, dim, page = [70, 33, 129], 128, 32
+    c = Cache(lens, kv_heads, dim, page=page, seed=21)
+    pages = c.keys.shape[0]
+    both = torch.full((pages, 2, kv_heads + 1, page, dim + 8), float("nan"), dtype=torch.bfloat16, device="cuda")
+    keys, values = both[:, 0, :kv_heads, :, :dim], both[:, 1, :kv_heads, :, :dim]
+    keys.copy_(c.keys), values.copy_(c.values)
+    h = tb.paged_cache(keys, values, c.table, mass=c.mass, positions=c.positions)
+    q, gate = query(c, 4 * kv_heads)
+    plain = c.clone()
+    out = torch.zeros_like(q)
+    ctx.attn_decode_paged(h, c.lanes, q, gate, out, scratch_for(h, 3, 129, 4 * kv_heads), max_keys=129)
+    assert torch.equal(out, decode(ctx, plain, q, gate, max_keys=129))
+    new = [torch.randn((3, kv_heads, dim), device="cuda").to(torch.bfloat16) for _ in range(2)]
+    ctx.paged_append(h, c.lanes, *new)
+    ctx.paged_append(handle(plain), plain.lanes, *new)
+    ctx.paged_evict(h, c.lanes, 40, torch.empty(tb.paged_evict_scratch_bytes(h, 3, 160, 40), dtype=torch.uint8, device="cuda"), sink=2, recent=9, max_keys=160)
+    run_evict(ctx, plain, 40, 2, 9)
+    ctx.sync()
+    assert same(keys, plain.keys) and same(values, plain.values) and same(c.mass, plain.mass) and same(c.positions, plain.positions)
+    assert torch.isnan(both[:, :, kv_heads:]).all() and torch.isnan(both[..., dim:]).all()
 
 
 def test_extreme_scores(ctx):
@@ -587,6 +613,37 @@ def test_a_served_batch_follows_its_definition(ctx, graph):
             assert same(c.rows(c.values, lane, head, n), model.rows(model.values, lane, head, n))
 
 
+def test_the_first_calls_of_a_process_inside_a_capture():
+    """Nothing has to be set up by an earlier call: a fresh process captures the operators at once and replays them."""
+    code = """
+import sys, torch
+sys.path.insert(0, %r), sys.path.insert(0, %r)
+import tatara_b200 as tb
+from paged_util import Cache, decode_definition
+ctx = tb.Context(0)
+c = Cache([200, 3000], 2, 256, seed=3)
+h = tb.paged_cache(c.keys, c.values, c.table, mass=c.mass, positions=c.positions)
+q, out = torch.randn((2, 16, 256), device="cuda").to(torch.bfloat16), torch.zeros((2, 16, 256), dtype=torch.bfloat16, device="cuda")
+want, bound, _, _ = decode_definition(c, q, None, 0.0625)
+scratch = torch.empty(tb.decode_paged_scratch_bytes(h, 2, h.capacity, 16), dtype=torch.uint8, device="cuda")
+trim = torch.empty(tb.paged_evict_scratch_bytes(h, 2, h.capacity, 150), dtype=torch.uint8, device="cuda")
+torch.cuda.synchronize()
+graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+with torch.cuda.graph(graph, stream=stream):
+    ctx.attn_decode_paged(h, c.lanes, q, None, out, scratch, stream=stream)
+    ctx.paged_evict(h, c.lanes, 150, trim, sink=4, recent=20, stream=stream)
+    ctx.paged_lanes_step(c.lanes, keep=150, advance=0, stream=stream)
+assert (out == 0).all()
+graph.replay()
+torch.cuda.synchronize()
+assert ((out.double() - want).abs() <= bound).all() and c.lanes[:, 0].tolist() == [150, 150]
+ctx.sync()
+print("captured")
+""" % (os.path.dirname(os.path.dirname(os.path.abspath(__file__))), os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_two_streams_at_once_and_a_stream_that_is_not_current(ctx):
     caches = [Cache([900, 40], 2, 256, seed=70 + i) for i in range(2)]
     asked = [query(c, 16) for c in caches]
@@ -619,7 +676,12 @@ def test_python_refusals(ctx):
                 lambda: ctx.paged_append(h, c.lanes, q[:, :2], gate[:, :2, :128]),
                 lambda: ctx.paged_append(h, c.lanes, q[:, :3], gate[:, :3]),
                 lambda: ctx.paged_append(h, c.lanes, q[:, :2], gate[:, :2], row_starts=c.lanes),
-                lambda: ctx.attn_qk_rope_paged(h, c.lanes, q, q, q, q, gate)):
+                lambda: ctx.attn_qk_rope_paged(h, c.lanes, q, q, q, q, gate),
+                lambda: ctx.attn_decode_paged(h, c.lanes, q, gate, out, scratch.cpu()),
+                lambda: ctx.attn_decode_paged(h, c.lanes.cpu(), q, gate, out, scratch),
+                lambda: ctx.attn_decode_paged(h, c.lanes, q.cpu(), gate, out, scratch),
+                lambda: ctx.paged_evict(h, c.lanes, 10, scratch.cpu()),
+                lambda: ctx.paged_append(h, c.lanes, q[:, :2].cpu(), gate[:, :2].cpu())):
         with pytest.raises(ValueError):
             bad()
     assert ctx.launches == launches
