@@ -430,13 +430,13 @@ class Context:
     @staticmethod
     def _paged_rows(what, t, cache, n, row):
         """n rows of `row` elements each in the cache's type, one stride apart; returns that stride."""
-        shape = t.shape
-        if shape[0] >= n and t.dtype is cache.torch_dtype and t.get_device() == cache.device:
-            if t.is_contiguous():
-                if t.numel() == shape[0] * row:
+        if t.dtype is cache.torch_dtype and t.get_device() == cache.device:
+            rows = t.size(0)
+            if rows >= n and t.numel() == rows * row:
+                if t.is_contiguous():
                     return row
-            elif t[0].numel() == row and t[0].is_contiguous():
-                return t.stride(0)
+                if t[0].is_contiguous():
+                    return t.stride(0)
         raise ValueError(f"{what}: at least {n} rows of {row} contiguous elements in the cache's type, on its device")
 
     @staticmethod
@@ -446,12 +446,11 @@ class Context:
         return scratch.data_ptr(), scratch.numel() * scratch.element_size()
 
     def _paged_lanes(self, lanes, cache=None):
-        _bind_torch()
-        shape = lanes.shape
-        if len(shape) != 2 or shape[1] != 2 or lanes.dtype is not _torch.int32 or not lanes.is_contiguous() or \
+        int32 = (_torch or _bind_torch()).int32
+        if lanes.dtype is not int32 or lanes.dim() != 2 or lanes.size(1) != 2 or not lanes.is_contiguous() or \
                 lanes.get_device() != self.device or cache is not None and cache.device != self.device:
             raise ValueError("lanes: [lane][2] int32, contiguous, on the context's device as the cache is")
-        return lanes.data_ptr(), shape[0]
+        return lanes.data_ptr(), lanes.size(0)
 
     def paged_append(self, cache, lanes, keys, values, row_starts=None, stream=None):
         """keys, values: [row][kv head][dim] views with one layout; row_starts: int32 [lanes + 1], or None for one row per lane."""

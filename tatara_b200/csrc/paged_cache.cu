@@ -100,6 +100,15 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 // loses its angle in f32 (2^18 / 1.6 has a last place of 1/64), then one sincospif; lanes 0 .. 7 take theirs by shuffles.
 constexpr uint32_t kRopeWarps = 4;
 
+// Turns of each pair from one position to the next; the model's divisors are base^(pair / 32) rounded to f32.
+struct RopeTurns {
+    double of[kRopePairs];
+    RopeTurns() {
+        for (uint32_t i = 0; i < kRopePairs; ++i)
+            of[i] = 1.0 / (6.283185307179586476925286766559 * double(static_cast<float>(std::pow(1.0e7, double(i) / 32.0))));
+    }
+};
+
 struct PagedRopeParams {
     PagedView cache;
     const tatara_paged_lane* lanes;
@@ -110,7 +119,7 @@ struct PagedRopeParams {
     __nv_bfloat16* gate_out;
     uint64_t projection_stride, query_stride;
     uint32_t n_lanes;
-    double turns[kRopePairs];   // turns of a pair from one position to the next
+    RopeTurns turns;
 };
 
 __device__ __forceinline__ void unpack8(const uint4 raw, float (&out)[8]) {
@@ -150,7 +159,7 @@ paged_rope_kernel(const __grid_constant__ PagedRopeParams p) {
     for (uint32_t i = 0; i < 8; ++i) acc = fmaf(x[i], x[i], acc);
     acc = warp_sum(acc);
     const float inverse = 1.0f / sqrtf(acc / float(kHeadDim) + kRmsEps);
-    const double turns = double(l.y) * p.turns[lane];
+    const double turns = double(l.y) * p.turns.of[lane];
     float sine, cosine;
     sincospif(2.0f * float(turns - rint(turns)), &sine, &cosine);
     __nv_bfloat16 res[8];
@@ -254,9 +263,8 @@ extern "C" tatara_status tatara_attn_qk_rope_paged(tatara_ctx* ctx, void* stream
     p.projection_stride = projection_stride;
     p.query_stride = query_stride;
     p.n_lanes = n_lanes;
-    // the model's divisors are base^(pair / 32) rounded to f32
-    for (uint32_t i = 0; i < kRopePairs; ++i)
-        p.turns[i] = 1.0 / (6.283185307179586476925286766559 * double(static_cast<float>(std::pow(1.0e7, double(i) / 32.0))));
+    static const RopeTurns turns;
+    p.turns = turns;
     const DeviceGuard guard(ctx);
     const uint32_t units = n_lanes * (kQHeads + kKvHeads);
     (void)launch_staged(paged_rope_kernel, dim3((units + kRopeWarps - 1u) / kRopeWarps), kRopeWarps * 32u, 0u,
