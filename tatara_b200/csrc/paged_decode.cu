@@ -587,35 +587,40 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 
 // ---- the join -----------------------------------------------------------------------------
 // With a mass, the first `walkers` CTAs add the weights to it, kMassSpan slots of a kv head at a time; the others finish 64 dims of a
-// head each.
+// head each, or a head.
 constexpr uint32_t kMassSpan = 1024;
 
-// A piece is finished by the CTA, or by one warp where no lane has more than 16 partitions: the same additions in the same order, so
-// the form is free to follow from max_keys.
-template <typename T, int D, bool kByWarp>
+// How a piece is finished: 64 dims by a CTA (few heads: the shortest way), 64 dims by a warp (no lane has more than 16 partitions), or a whole
+// head by a CTA (many heads: a quarter of the CTAs, each weighing its partitions once).  The same additions in the same order, so the
+// form is free to follow from the call's bounds.
+enum JoinForm { kJoinSlice, kJoinWarp, kJoinHead };
+template <typename T, int D, JoinForm kForm>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t walkers) {
     __shared__ uint32_t item_start[TATARA_MAX_LANES + 1], lane_keys[TATARA_MAX_LANES], warp_total[kJoinWarps];
     __shared__ float weight[kSmCount * 2];                 // per_wave at most
     __shared__ float red[kJoinWarps], red_sum[kJoinWarps];
-    __shared__ __align__(16) float acc_s[kJoinPhases][kJoinDims];
+    constexpr uint32_t kWidth = kForm == kJoinHead ? D : kJoinDims;             // dims of a piece
+    __shared__ __align__(16) float acc_s[kJoinPhases][kWidth];
     __shared__ float2 final_ml[16];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    constexpr uint32_t kSlices = D / kJoinDims;
+    constexpr uint32_t kSlices = D / kWidth;
     wait_for_predecessor();
     release_dependents();
     if (blockIdx.x >= walkers) {
-        const uint32_t piece = kByWarp ? (blockIdx.x - walkers) * kJoinWarps + warp : blockIdx.x - walkers;
+        const uint32_t piece = kForm == kJoinWarp ? (blockIdx.x - walkers) * kJoinWarps + warp : blockIdx.x - walkers;
         const uint32_t slice = piece % kSlices, rest = piece / kSlices, head = rest % p.q_heads, row = rest / p.q_heads;
         if (row >= p.n_lanes) return;
         const uint32_t n = __ldcg(&p.lanes[row].keys);
         if (n > p.max_keys) return;                        // refused: its row stays as it is
         const uint32_t parts = n == 0u ? 0u : p.cut.parts(n);
         const uint64_t record = (uint64_t(row) * p.q_heads + head) * p.parts;
-        const uint32_t pair = lane, phase = warp;
-        const float* base = p.sums + record * D + slice * kJoinDims + pair * 2u;
-        const uint64_t out_row = row * p.query_stride + uint64_t(head) * D + slice * kJoinDims;
-        if constexpr (kByWarp) {
+        // a thread owns two dims and kOwn of the phases
+        constexpr uint32_t kColumns = kWidth / 2u, kOwn = kJoinPhases * kColumns / kJoinThreads;
+        const uint32_t pair = threadIdx.x % kColumns, phase = threadIdx.x / kColumns * kOwn;
+        const float* base = p.sums + record * D + slice * kWidth + pair * 2u;
+        const uint64_t out_row = row * p.query_stride + uint64_t(head) * D + slice * kWidth;
+        if constexpr (kForm == kJoinWarp) {
             const uint64_t at = (out_row + pair * 2u) * 2u;
             float gate0 = 0.0f, gate1 = 0.0f;
             if (p.gate != nullptr) {
@@ -664,15 +669,20 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
         }
         const uint64_t at = (out_row + threadIdx.x) * 2u;
         float gate = 0.0f;
-        if (threadIdx.x < kJoinDims && p.gate != nullptr) gate = Half<T>::load(p.gate + at);
+        if (threadIdx.x < kWidth && p.gate != nullptr) gate = Half<T>::load(p.gate + at);
         // the first partitions' sums are asked for before their weights are known
-        constexpr uint32_t kAhead = 10;
-        float2 v[kAhead];
+        constexpr uint32_t kAhead = kOwn == 1u ? 10u : 3u;
+        float2 v[kAhead][kOwn];
+        auto ask = [&](uint32_t round0) {
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t part = phase + i * kJoinPhases;
-            v[i] = part < parts ? __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D)) : make_float2(0.0f, 0.0f);
-        }
+            for (uint32_t i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (uint32_t f = 0; f < kOwn; ++f) {
+                    const uint32_t part = (round0 + i) * kJoinPhases + phase + f;
+                    if (part < parts) v[i][f] = __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D));
+                }
+        };
+        ask(0u);
         static_assert(kSmCount * 2u <= 2u * kJoinThreads, "two partitions a thread");
         float2 ml[2];
 #pragma unroll
@@ -700,23 +710,26 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
         for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         if (lane == 0) red_sum[warp] = sum;
         __syncthreads();
-        float a0 = 0.0f, a1 = 0.0f;
+        float2 a[kOwn];
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t part = phase + i * kJoinPhases;
-            if (part < parts) {
-                a0 = fmaf(weight[part], v[i].x, a0);
-                a1 = fmaf(weight[part], v[i].y, a1);
-            }
+        for (uint32_t f = 0; f < kOwn; ++f) a[f] = make_float2(0.0f, 0.0f);
+        for (uint32_t round0 = 0; round0 * kJoinPhases < parts; round0 += kAhead) {
+            if (round0 != 0u) ask(round0);
+#pragma unroll
+            for (uint32_t i = 0; i < kAhead; ++i)
+#pragma unroll
+                for (uint32_t f = 0; f < kOwn; ++f) {
+                    const uint32_t part = (round0 + i) * kJoinPhases + phase + f;
+                    if (part < parts) {
+                        a[f].x = fmaf(weight[part], v[i][f].x, a[f].x);
+                        a[f].y = fmaf(weight[part], v[i][f].y, a[f].y);
+                    }
+                }
         }
-        for (uint32_t part = phase + kAhead * kJoinPhases; part < parts; part += kJoinPhases) {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(base + uint64_t(part) * D));
-            a0 = fmaf(weight[part], x.x, a0);
-            a1 = fmaf(weight[part], x.y, a1);
-        }
-        *reinterpret_cast<float2*>(&acc_s[phase][pair * 2u]) = make_float2(a0, a1);
+#pragma unroll
+        for (uint32_t f = 0; f < kOwn; ++f) *reinterpret_cast<float2*>(&acc_s[phase + f][pair * 2u]) = a[f];
         __syncthreads();
-        if (threadIdx.x < kJoinDims) {
+        if (threadIdx.x < kWidth) {
             float num = 0.0f, den = 0.0f;
 #pragma unroll
             for (uint32_t ph = 0; ph < kJoinPhases; ++ph) num += acc_s[ph][threadIdx.x];
@@ -834,9 +847,11 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     const uint64_t spans = uint64_t(p.n_lanes) * p.cache.kv_heads * ((p.max_keys + kMassSpan - 1u) / kMassSpan);
     const uint32_t walkers = p.cache.mass == nullptr ? 0u : uint32_t(spans < 4u * ctx->sm_count ? spans : 4u * ctx->sm_count);
     if (p.parts <= 16u)
-        (void)launch_staged(paged_join_kernel<T, D, true>, dim3((pieces + kJoinWarps - 1u) / kJoinWarps + walkers), kJoinThreads, 0u, stream, p, walkers);
+        (void)launch_staged(paged_join_kernel<T, D, kJoinWarp>, dim3((pieces + kJoinWarps - 1u) / kJoinWarps + walkers), kJoinThreads, 0u, stream, p, walkers);
+    else if (D != 64 && pieces > 4u * sms)
+        (void)launch_staged(paged_join_kernel<T, D, kJoinHead>, dim3(p.n_lanes * p.q_heads + walkers), kJoinThreads, 0u, stream, p, walkers);
     else
-        (void)launch_staged(paged_join_kernel<T, D, false>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
+        (void)launch_staged(paged_join_kernel<T, D, kJoinSlice>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
     return check_launch(ctx, "attn_decode_paged: join");
 }
 

@@ -114,7 +114,7 @@ def test_the_longest_context(ctx):
     assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
 
 
-@pytest.mark.parametrize("dim,kv_heads,group", [(256, 2, 8), (128, 4, 12), (64, 3, 5)])
+@pytest.mark.parametrize("dim,kv_heads,group", [(256, 2, 8), (256, 7, 6), (128, 4, 12), (128, 16, 6), (64, 3, 5)])
 def test_a_lane_has_the_same_bits_alone_in_a_batch_and_in_other_pages(ctx, dim, kv_heads, group):
     lens = [700, 0, 1300, 90, 12000, 257]
     c = Cache(lens, kv_heads, dim, seed=4)
