@@ -502,8 +502,8 @@ typedef struct tatara_paged_cache {
  * (so a contiguous lane cache [kv head][capacity][dim] is a source as it is).  row_starts: device,
  * [n_lanes + 1], ascending from 0; rows from row_starts[n_lanes] up to n_rows (padding) are not read.
  * row_starts == NULL: row i belongs to lane i (n_rows == n_lanes).  The slots' mass is set to 0 and their
- * positions to the tokens'.  A row whose slot would lie before slot 0 or beyond the page table is left out and
- * latches TATARA_CONTEXT_OUT_OF_RANGE. */
+ * positions to the tokens'.  A row whose slot would lie before slot 0 or beyond the page table is left out, and so
+ * are rows that row_starts counts beyond n_rows; either latches TATARA_CONTEXT_OUT_OF_RANGE. */
 tatara_status tatara_paged_append(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
                                   const tatara_paged_lane* lanes_device, uint32_t n_lanes, const void* keys,
                                   const void* values, uint64_t row_stride, uint64_t source_head_stride,

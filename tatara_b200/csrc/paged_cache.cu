@@ -53,6 +53,8 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
     extern __shared__ __align__(16) uint8_t append_smem[];
     uint64_t* dst = reinterpret_cast<uint64_t*>(append_smem);   // [tile_rows]: byte offset of head 0's row, ~0 = none
     wait_for_predecessor();
+    if (blockIdx.x == 0u && threadIdx.x == 0u && p.row_starts != nullptr && __ldcg(p.row_starts + p.n_lanes) > p.n_rows)
+        latch_out_of_range(p.cache, p.n_lanes);   // rows that were promised and are not there
     const uint32_t first = blockIdx.x * p.tile_rows, rows = min(p.tile_rows, p.n_rows - first), heads = p.cache.kv_heads;
     for (uint32_t r = threadIdx.x; r < rows; r += kAppendThreads) {
         uint32_t lane, slot, position;

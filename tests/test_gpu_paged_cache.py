@@ -104,6 +104,40 @@ def test_many_short_lanes(ctx, kv_heads, group, dim, most):
     assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
 
 
+def test_more_partitions_than_a_cta_describes_at_once(ctx):
+    """256 lanes of 300 heads are about 260 partitions for every CTA; the same lanes in calls of eight are at most nine."""
+    rng = np.random.default_rng(8)
+    lens = [int(x) for x in rng.integers(0, 17, 256)]
+    lens[7], lens[200] = 16, 1
+    c = Cache(lens, 300, 256, page=16, seed=8, extra_columns=0)
+    q, gate = query(c, 300)
+    out = decode(ctx, c, q, gate, mass=False)
+    for i in range(0, 256, 8):
+        part = tb.paged_cache(c.keys, c.values, c.table[i: i + 8])
+        got, lanes = torch.full_like(q[i: i + 8], 7.0), c.lanes[i: i + 8].contiguous()
+        ctx.attn_decode_paged(part, lanes, q[i: i + 8], gate[i: i + 8], got, scratch_for(part, 8, 16, 300))
+        ctx.sync()
+        assert torch.equal(got, out[i: i + 8])
+
+
+def test_lanes_that_share_a_prefix(ctx):
+    """Two lanes on the same first pages: decode reads them twice, the masses stay apart, an eviction that guards the prefix leaves it."""
+    c = Cache([200, 150], 2, 128, page=16, seed=33)
+    c.table[1, :4] = c.table[0, :4]                                   # 64 common slots
+    q, gate = query(c, 8)
+    want, bound, added, added_bound = decode_definition(c, q, gate, 128 ** -0.5)
+    before = c.mass.double()
+    out = decode(ctx, c, q, gate)
+    assert ((out.double() - want).abs() <= bound).all()
+    assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
+    # each lane against a definition of its own cache: no page below the guarded slots is written
+    prefix = [x[c.table[0, :4].long()].clone() for x in (c.keys, c.values)]
+    expected = evict_definition(c, 100, 64, 12)
+    run_evict(ctx, c, 100, 64, 12)
+    assert same_cache(c, expected)
+    assert all(same(x[c.table[0, :4].long()], y) for x, y in zip((c.keys, c.values), prefix))
+
+
 def test_the_longest_context(ctx):
     c = Cache([262144], 2, 256, page=64, seed=9, extra_columns=0)
     q, gate = query(c, 16)
@@ -301,6 +335,21 @@ def test_append_leaves_out_what_has_no_slot(ctx):
         want.keys[page, :, slot % 16], want.values[page, :, slot % 16] = k[row], v[row]
         want.mass[lane, :, slot], want.positions[lane, :, slot] = 0.0, slot
     ctx.paged_append(handle(c), c.lanes, k, v, row_starts=torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    with pytest.raises(tb.TataraError) as e:
+        ctx.sync()
+    assert e.value.status == RANGE
+    assert same_cache(c, want)
+
+
+def test_append_of_rows_that_are_not_there(ctx):
+    c = Cache([40, 40], 1, 64, seed=4)
+    k, v = (torch.randn((50, 1, 64), device="cuda").to(torch.bfloat16) for _ in range(2))
+    want = append_definition(c, [0, 40, 80], torch.cat([k, k]), torch.cat([v, v]))
+    for slot in range(10, 40):                                        # rows 50 .. 79 of lane 1 are missing
+        page, row = int(c.table[1, slot // 16]), slot % 16
+        want.keys[page, :, row], want.values[page, :, row] = c.keys[page, :, row], c.values[page, :, row]
+        want.mass[1, :, slot], want.positions[1, :, slot] = c.mass[1, :, slot], c.positions[1, :, slot]
+    ctx.paged_append(handle(c), c.lanes, k, v, row_starts=torch.tensor([0, 40, 80], dtype=torch.int32, device="cuda"))
     with pytest.raises(tb.TataraError) as e:
         ctx.sync()
     assert e.value.status == RANGE
