@@ -92,7 +92,7 @@ uint64_t tatara_ctx_launch_count(const tatara_ctx* ctx);
 typedef enum tatara_policy {
     /* Cap on the rows of K and of V of each decode CTA's partition that are requested into L2 before
      * the kernel waits for its predecessor in the stream (the kernel asks for a quarter of the
-     * partition up to this cap; 0 switches the requests off). */
+     * partition up to this cap; 0 switches the requests off).  Holds for tatara_attn_decode_paged too. */
     TATARA_POLICY_DECODE_L2_PREFETCH_KEYS = 0,
     /* Which implementation evaluates tatara_gdn_prefill with chunk 64: 0 = the tensor-memory form
      * (tcgen05 MMAs fed by TMA, the state as an f32 accumulator in tensor memory) as ONE launch in which

@@ -64,6 +64,7 @@ struct PagedDecodeParams {
     uint32_t parts;        // parts of the longest lane: the stride of sums and stats
     uint32_t score_slots;  // max_keys rounded up to 16
     uint32_t units;        // places of a warp's ring
+    uint32_t ahead_slots;  // most slots of a partition asked into L2 before the predecessor is waited for
     uint32_t page_slices, page_magic;   // slices of a page; floor(2^32 / page_slices) + 1
     float scale_log2e;
 };
@@ -186,7 +187,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// kTiles: tiles of eight query heads, 1 or 2.
+// kTiles: tiles of eight query heads, 1 or 2.  Measured with the join, 2 kv heads of 256, 16 query heads, bf16: one lane of 262144 slots 84 us
+// (6.3 TB/s of K and V, bound by HBM), of 4096 9.3 us (latency), 32 lanes of 16384 185 us (5.8 TB/s); 16 lanes of 8192, 8 kv heads of
+// 128 91 us (5.9 TB/s), of 64 51 us (5.2 TB/s, bound by the instructions of a step).
 template <typename T, int D, int kTiles>
 __global__ void __launch_bounds__(kPdThreads, pd_ctas(D, kTiles == 2))
 paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
@@ -202,6 +205,38 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     uint32_t* warp_word = lane_keys + TATARA_MAX_LANES;
     const uint32_t ring = smem_u32(smem + warp * p.units * G::kUnit);
     const uint64_t policy = l2_evict_first_policy();
+    // Before the predecessor is waited for, the first rows of this CTA's partition are asked into L2, so that HBM streams across the boundary
+    // of the kernels.  The lane and the page table may be changing meanwhile; whatever they say, only rows inside the pools are asked for,
+    // nothing lands in registers or shared memory, and both are read again after the wait.  Only where a CTA has one partition:
+    // a batch keeps HBM busy by itself.
+    if constexpr (kTiles == 1) {
+        if (p.ahead_slots != 0u) {
+            scan_items<kPdThreads>(p, item_start, lane_keys, warp_word, false, [&](uint32_t n) { return p.cut.parts(n); });
+            if (blockIdx.x < item_start[p.n_lanes]) {
+                const PagedItem it = item_at(p, item_start, lane_keys, blockIdx.x, [&](uint32_t n) { return p.cut.part_slots(n); });
+                // a quarter of the partition at most: more competes in L2 with what is still streaming
+                const uint32_t slices = min(p.ahead_slots, (it.slots + 3u) / 4u + kPagedSlice - 1u) / kPagedSlice;
+                for (uint32_t s = threadIdx.x; s < slices; s += kPdThreads) {
+                    const uint32_t slice = it.begin / kPagedSlice + s;
+                    const uint32_t column = p.page_slices == 1u ? slice : __umulhi(slice, p.page_magic);
+                    const uint32_t page = __ldcg(p.cache.page_table + uint64_t(it.lane) * p.cache.table_pages + column);
+                    if (page >= p.cache.n_pages) continue;
+                    const uint32_t rows = min(kPagedSlice, it.slots - s * kPagedSlice);
+                    const uint64_t offset = page * p.cache.page_bytes + it.kv * p.cache.head_bytes + (slice - column * p.page_slices) * kPagedSlice * p.cache.slot_bytes;
+                    if (p.cache.slot_bytes == G::kRow) {
+                        l2_prefetch_bulk(p.cache.keys + offset, rows * G::kRow);
+                        l2_prefetch_bulk(p.cache.values + offset, rows * G::kRow);
+                    } else {
+                        for (uint32_t r = 0; r < rows; ++r) {
+                            l2_prefetch_bulk(p.cache.keys + offset + r * p.cache.slot_bytes, G::kRow);
+                            l2_prefetch_bulk(p.cache.values + offset + r * p.cache.slot_bytes, G::kRow);
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+        }
+    }
     wait_for_predecessor();
     release_dependents();
     scan_items<kPdThreads>(p, item_start, lane_keys, warp_word, blockIdx.x == 0, [&](uint32_t n) { return p.cut.parts(n); });
@@ -588,6 +623,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
 // ---- the join -----------------------------------------------------------------------------
 // With a mass, the first `walkers` CTAs add the weights to it, kMassSpan slots of a kv head at a time; the others finish 64 dims of a
 // head each, or a head.
+// Bound by latency for a lane alone (3 us behind the first kernel), by L2 in a batch (records, scores and mass of 32 lanes of 4096 to
+// 32768 slots: 10 us).
 constexpr uint32_t kMassSpan = 1024;
 
 // How a piece is finished: 64 dims by a CTA (few heads: the shortest way), 64 dims by a warp (no lane has more than 16 partitions), or a whole
@@ -840,6 +877,9 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, sms = ctx->sm_count;
     const uint32_t ctas = items >= kCtas * sms ? kCtas : uint32_t((items + sms - 1u) / sms);   // on an SM
     p.units = G::units(ctas);
+    // Asking ahead pays for long partitions (one lane of 262144 slots 86.5 -> 83.3 us, of 131072 with head_dim 128 49 -> 45), costs 0.2 us
+    // where they are the shortest, and slows the arithmetic-bound wide groups (28 -> 32 us).
+    p.ahead_slots = items <= kCtas * sms && kTiles == 1 && p.cut.part_slots(p.max_keys) > p.cut.least ? ctx->decode_l2_prefetch_keys : 0u;
     (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < kCtas * sms ? items : kCtas * sms)), kPdThreads, G::smem(p.units, kTiles == 2), stream, p);
     const tatara_status st = check_launch(ctx, "attn_decode_paged");
     if (st != TATARA_OK) return st;

@@ -168,6 +168,32 @@ def test_a_lane_has_the_same_bits_alone_in_a_batch_and_in_other_pages(ctx, dim, 
         assert same(alone.mass[0, :, :n], batch_mass[i, :, :n])
 
 
+@pytest.mark.parametrize("slot_major,dim", [(False, 256), (True, 128), (True, 64)])
+def test_rows_asked_ahead_change_no_bit(ctx, slot_major, dim):
+    """Long partitions ask their first rows into L2 before the wait; tokens whose lane and rows change right before each call."""
+    n, kept = 60000, ctx.get_policy(tb.POLICY_DECODE_L2_PREFETCH_KEYS)
+    c = Cache([n + 40], 2, dim, page=64, slot_major=slot_major, seed=dim)
+    c.lanes[0, 0] = n
+    q, gate = query(c, 8)
+    rows = [torch.randn((40, 1, 2, dim), device="cuda").to(torch.bfloat16) for _ in range(2)]
+    results = []
+    for ahead in (0, 512):
+        ctx.set_policy(tb.POLICY_DECODE_L2_PREFETCH_KEYS, ahead)
+        own = c.clone()
+        h = handle(own)
+        scratch, outs = scratch_for(h, 1, h.capacity, 8), torch.zeros((40, *q.shape), dtype=q.dtype, device="cuda")
+        torch.cuda.synchronize()
+        for i in range(40):
+            ctx.paged_lanes_step(own.lanes)
+            ctx.paged_append(h, own.lanes, rows[0][i], rows[1][i])
+            ctx.attn_decode_paged(h, own.lanes, q, gate, outs[i], scratch)
+        ctx.sync()
+        results.append((outs, own))
+    ctx.set_policy(tb.POLICY_DECODE_L2_PREFETCH_KEYS, kept)
+    assert torch.equal(results[0][0], results[1][0]) and same_cache(results[0][1], results[1][1])
+    assert torch.isfinite(results[0][0]).all()
+
+
 def test_matches_the_contiguous_decode(ctx):
     """The same cache as a stripe of the contiguous operator: two results within both operators' roundings."""
     n = 3001
