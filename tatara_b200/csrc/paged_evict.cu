@@ -69,6 +69,9 @@ __global__ void __launch_bounds__(kSelThreads, 1)
 paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
     __shared__ __align__(16) SelectShared s;
     cg::cluster_group cluster = cg::this_cluster();
+    const auto meet = [&] {            // the CTAs that share a head
+        if (p.cluster == 1u) __syncthreads(); else cluster.sync();
+    };
     const uint32_t rank = blockIdx.x % p.cluster, row = blockIdx.x / p.cluster;
     const uint32_t lane_row = row / p.cache.kv_heads, head = row - lane_row * p.cache.kv_heads;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -134,7 +137,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
                 atomicAdd(&s.hist[digit][bin], 1u);
             }
         }
-        cluster.sync();
+        meet();
         if (p.cluster == 1u) {
             // thread t takes bins 2t and 2t + 1, counted from the top
             const uint32_t top = bins - 2u - threadIdx.x * 2u;
@@ -209,7 +212,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
     uint4 b = make_uint4(__shfl_sync(0xffffffffu, sum.x, prior), __shfl_sync(0xffffffffu, sum.y, prior), __shfl_sync(0xffffffffu, sum.z, prior),
                          __shfl_sync(0xffffffffu, sum.w, prior));
     if (warp == 0u) b = make_uint4(0u, 0u, 0u, 0u);
-    cluster.sync();
+    meet();
     const uint4 other = lane < p.cluster ? *cluster.map_shared_rank(&s.counts, lane) : make_uint4(0u, 0u, 0u, 0u);
     const bool prior_rank = lane < rank;
     b.x += __reduce_add_sync(0xffffffffu, prior_rank ? other.x : 0u);
@@ -267,7 +270,7 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
             donor_at += __popc(db);
         }
     }
-    cluster.sync();   // nobody leaves while its counters are read
+    if (p.cluster != 1u) cluster.sync();   // nobody leaves while its counters are read
 }
 
 // A warp takes p.warp_pairs pairs: each lane looks up one pair's slots and pages, then kChunks lanes together copy a pair's rows, with
