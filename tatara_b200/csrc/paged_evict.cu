@@ -60,8 +60,8 @@ __device__ __forceinline__ uint32_t warp_inclusive(uint32_t v) {
     return v;
 }
 
-// Measured: 8 us for two heads of 4196 slots, 23 us for two of 262144 (32 SMs; a digit's step 4.5 us, of which 2.6 are spent between the
-// CTAs), 21 us for 192 heads of up to 16000.
+// Measured: 7 us for two heads of 4196 slots, 23 us for two of 262144 (32 SMs; a digit's step 4.5 us, of which 2.6 are spent between the
+// CTAs), 19 us for 192 heads of up to 16000.
 // kKeys: the most keys of a thread; `each` of them are used, as many as the lane's slots need.  A warp owns a run of 32 * each slots,
 // lane by lane, so ballots count in the order of the slots.
 template <uint32_t kKeys>
