@@ -22,11 +22,11 @@
  *     (src/runtime/decode_step.cpp:812-824); a failing call enqueues nothing.
  *   - Calls are asynchronous on `stream`; errors of earlier asynchronous work surface
  *     as TATARA_CUDA_ERROR from a later call or from tatara_ctx_sync.
- *   - The kernels that use thread-block clusters (tatara_attn_prefill and tatara_project_dense, with
- *     tensor memory; tatara_paged_evict where max_keys is above 16384) are issued with nothing else of
- *     this library in flight on the device: keep them in the stream that carries the rest of the work.
- *     Issued beside other streams' kernels the first two have stalled (cause not established); the host
- *     layer's owner loop (tatara_b200/host/wave_loop.hpp) therefore uses one stream.
+ *   - The block kernels that use thread-block clusters and tensor memory (tatara_attn_prefill,
+ *     tatara_project_dense) are issued with nothing else of this library in flight on the
+ *     device: keep them in the stream that carries the rest of the work.  Issued beside other
+ *     streams' kernels they have stalled (cause not established); the host layer's owner loop
+ *     (tatara_b200/host/wave_loop.hpp) therefore uses one stream.
  */
 #ifndef TATARA_B200_H_
 #define TATARA_B200_H_
@@ -471,8 +471,7 @@ tatara_status tatara_lanes_advance(tatara_ctx* ctx, void* stream, tatara_attn_la
  * as they are), a page number >= n_pages is neither read nor written (its slots count as absent); either
  * latches TATARA_CONTEXT_OUT_OF_RANGE for the next tatara_ctx_sync.  Lanes with keys == 0 are idle.
  * Calls on different streams may run at the same time as long as they share no scratch and none writes
- * what another touches -- except tatara_paged_evict with max_keys above 16384 (the rule on cluster kernels
- * at the head of this file).  Calls switch to the context's device and back. */
+ * what another touches.  Calls switch to the context's device and back. */
 typedef enum tatara_dtype { TATARA_BF16 = 0, TATARA_F16 = 1 } tatara_dtype;
 #define TATARA_MAX_GROUP 16u /* query heads per kv head of the paged decode */
 

@@ -170,8 +170,8 @@ struct PdGeometry {
     static constexpr uint32_t kMaxUnits = 6;
     static constexpr uint32_t query(bool wide) { return wide ? 16u * kRow : 0u; }   // sixteen heads do not fit in registers beside their sums
     static constexpr uint32_t smem(uint32_t units, bool wide) { return query(wide) + kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
-    // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and the rest of the SM's memory
-    // serves the copies better as L1 than as a deeper ring.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings an SM, 93 - 99 at
+    // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and more shared memory slows the
+    // stream down, most likely because it comes out of L1, which the copies pass.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings an SM, 93 - 99 at
     // 160 to 192; 32 lanes of 16384: 189 us at 128 KiB, 205 at 192.
     static constexpr uint32_t units(uint32_t ctas) {
         const uint32_t u = 1u + 64u * 1024u / (ctas * kPdWarps * kUnit);
