@@ -546,7 +546,7 @@ def test_evict_matches_the_definition(ctx, kind, lens, keep, sink, recent):
     (2, 256, 4200, 4096, 4, 100, "spread"), (2, 128, 20000, 5000, 64, 1000, "ties"), (1, 64, 52001, 1000, 0, 0, "spread"),
     (1, 64, 262144, 100000, 128, 4096, "ties"), (40, 64, 5000, 2500, 3, 7, "odd"), (160, 64, 300, 100, 1, 5, "spread")])
 def test_evict_of_long_lanes_and_many_heads(ctx, kv_heads, dim, n, keep, sink, recent, kind):
-    """Every size of the search's clusters, from one CTA for a head to eight."""
+    """A CTA for a head with 2 to 16 keys a thread, and lanes that many CTAs share."""
     c = Cache([n], kv_heads, dim, page=64, seed=n, extra_columns=0)
     fill_mass(c, kind)
     # slots in no order of position, as after earlier evictions
@@ -554,6 +554,34 @@ def test_evict_of_long_lanes_and_many_heads(ctx, kv_heads, dim, n, keep, sink, r
     want = evict_definition(c, keep, sink, recent)
     run_evict(ctx, c, keep, sink, recent)
     assert same_cache(c, want)
+
+
+@pytest.mark.parametrize("kv_heads,lens,keep,sink,recent,kind", [
+    (16, [40000, 700, 16385, 30001], 700, 3, 40, "spread"), (13, [17000, 20480, 20481, 9], 16384, 5, 2000, "ties"), (2, [16385, 36865, 0], 4096, 0, 0, "equal"),
+    (3, [70000, 50, 33000], 30000, 9, 100, "odd")])
+def test_evict_of_ragged_long_lanes(ctx, kv_heads, lens, keep, sink, recent, kind):
+    """Lanes of many CTAs next to lanes of one and lanes that stay, in few large and many small shares; a lane beyond max_keys is left alone."""
+    c = Cache(lens, kv_heads, 64, page=64, seed=keep, extra_columns=0)
+    fill_mass(c, kind)
+    for lane, n in enumerate(lens):
+        c.positions[lane, :, :n] = torch.stack([torch.randperm(n, generator=c.gen, device="cuda") for _ in range(kv_heads)]).to(torch.int32)
+    want = evict_definition(c, keep, sink, recent)
+    before = c.clone()
+    run_evict(ctx, c, keep, sink, recent)
+    assert same_cache(c, want)
+    h = handle(before)
+    untouched = before.clone()
+    most = max(x for x in lens if x < max(lens))
+    scratch = torch.full((tb.paged_evict_scratch_bytes(h, len(lens), most, keep),), 0x5A, dtype=torch.uint8, device="cuda")
+    ctx.paged_evict(h, before.lanes, keep, scratch, sink=sink, recent=recent, max_keys=most)
+    with pytest.raises(tb.TataraError) as e:
+        ctx.sync()
+    assert e.value.status == RANGE
+    long = lens.index(max(lens))
+    mine = untouched.table[long].long()
+    assert same(before.keys[mine], untouched.keys[mine]) and same(before.mass[long], untouched.mass[long])
+    rest = [i for i in range(len(lens)) if i != long]
+    assert all(same(before.mass[i], want.mass[i]) and same(before.keys[want.table[i].long()], want.keys[want.table[i].long()]) for i in rest)
 
 
 def test_evict_more_guarded_than_kept(ctx):
