@@ -765,6 +765,27 @@ def test_two_streams_at_once_and_a_stream_that_is_not_current(ctx):
         assert torch.equal(got, expected)
 
 
+def test_an_eviction_beside_a_decode_on_another_stream(ctx):
+    """A long lane is trimmed on one stream while another batch decodes on a second one; each finds what it finds alone."""
+    trimmed, batch = Cache([40000, 20000], 2, 64, page=64, seed=80), Cache([3000, 700, 1], 2, 256, seed=81)
+    fill_mass(trimmed, "spread")
+    want = evict_definition(trimmed, 9000, 4, 500)
+    q, gate = query(batch, 16)
+    expected = decode(ctx, batch.clone(), q, gate, mass=False)
+    h, hb = handle(trimmed), handle(batch, mass=False)
+    trim = torch.empty(tb.paged_evict_scratch_bytes(h, 2, h.capacity, 9000), dtype=torch.uint8, device="cuda")
+    scratch, outs = scratch_for(hb, 3, hb.capacity, 16), torch.zeros((30, *q.shape), dtype=q.dtype, device="cuda")
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(30):
+        ctx.attn_decode_paged(hb, batch.lanes, q, gate, outs[i], scratch, stream=streams[0])
+        if i == 10:
+            ctx.paged_evict(h, trimmed.lanes, 9000, trim, sink=4, recent=500, stream=streams[1])
+    torch.cuda.synchronize()
+    ctx.sync()
+    assert same_cache(trimmed, want) and all(torch.equal(o, expected) for o in outs)
+
+
 def test_python_refusals(ctx):
     c = Cache([10, 20], 2, 256, seed=1)
     h = handle(c)
