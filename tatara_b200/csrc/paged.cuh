@@ -99,20 +99,28 @@ struct DeviceGuard {
     }
 };
 
-// A launch that may be staged while its predecessor in the stream finishes (the kernel waits for it itself).
+// A launch that may be staged while its predecessor in the stream finishes (the kernel waits for it itself).  carveout: the share
+// of an SM's memory, in percent, that is to be shared memory; -1: the driver's choice.
 template <typename... Params, typename... Args>
-inline cudaError_t launch_staged(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, Args&&... args) {
-    cudaLaunchAttribute attr[1];
+inline cudaError_t launch_staged_carved(int carveout, void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream,
+                                        Args&&... args) {
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributePreferredSharedMemoryCarveout;
+    attr[1].val.sharedMemCarveout = uint32_t(carveout);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = carveout < 0 ? 1 : 2;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+template <typename... Params, typename... Args>
+inline cudaError_t launch_staged(void (*kernel)(Params...), dim3 grid, uint32_t threads, uint32_t smem, cudaStream_t stream, Args&&... args) {
+    return launch_staged_carved(-1, kernel, grid, threads, smem, stream, static_cast<Args&&>(args)...);
 }
 __device__ __forceinline__ void wait_for_predecessor() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

@@ -27,8 +27,9 @@ constexpr uint32_t kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinDims
 constexpr uint32_t kJoinPhases = 8;           // the join adds partitions f, f + 8, ... in phase f, then the phases in order
 
 // CTAs of the first kernel that share an SM: their rings fill its shared memory, their accumulators its registers.  Several, so
-// that one streams while another joins its warps, fetches a query or looks up a page.
-__host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim, bool wide) { return head_dim == 256u ? 2u : head_dim == 128u && wide ? 3u : 4u; }
+// that one streams while another joins its warps, fetches a query or looks up a page.  Four need 128 registers a thread, which head_dim 128
+// does not fit in: 64 lanes of 1024 slots 56 us with four, 51 with three; one of 4096 9.6 and 8.8.
+__host__ __device__ constexpr uint32_t pd_ctas(uint32_t head_dim) { return head_dim == 256u ? 2u : head_dim == 128u ? 3u : 4u; }
 // The cut of a lane of n slots: partitions of at least pd_min_part slots, and no more items than one CTA for each SM (head_dim 256) or two
 // take in one go.  Fewer and longer ones serve a batch better (fewer records), more of them would only help a lane alone.
 __host__ __device__ inline uint32_t pd_per_wave(uint32_t kv_heads, uint32_t head_dim) {
@@ -171,8 +172,8 @@ struct PdGeometry {
     static constexpr uint32_t query(bool wide) { return wide ? 16u * kRow : 0u; }   // sixteen heads do not fit in registers beside their sums
     static constexpr uint32_t smem(uint32_t units, bool wide) { return query(wide) + kPdWarps * units * kUnit + kPdItems * 16 + kPdWarps * 8 * 8 + (2 * TATARA_MAX_LANES + 16) * 4; }
     // Places of a warp's ring when `ctas` share an SM: 64 KiB in flight an SM carry the full rate (6 TB/s), and more shared memory slows the
-    // stream down, most likely because it comes out of L1, which the copies pass.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings an SM, 93 - 99 at
-    // 160 to 192; 32 lanes of 16384: 189 us at 128 KiB, 205 at 192.
+    // stream down, most likely because it comes out of L1, which the copies pass.  One lane of 262144 slots: 88 us at 96 to 128 KiB of rings
+    // an SM, 93 - 99 at 160 to 192; 32 lanes of 16384: 189 us at 128 KiB, 205 at 192.
     static constexpr uint32_t units(uint32_t ctas) {
         const uint32_t u = 1u + 64u * 1024u / (ctas * kPdWarps * kUnit);
         return u < 2u ? 2u : u > kMaxUnits ? kMaxUnits : u;
@@ -191,7 +192,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // (6.3 TB/s of K and V, bound by HBM), of 4096 9.3 us (latency), 32 lanes of 16384 185 us (5.8 TB/s); 16 lanes of 8192, 8 kv heads of
 // 128 91 us (5.9 TB/s), of 64 51 us (5.2 TB/s, bound by the instructions of a step).
 template <typename T, int D, int kTiles>
-__global__ void __launch_bounds__(kPdThreads, pd_ctas(D, kTiles == 2))
+__global__ void __launch_bounds__(kPdThreads, pd_ctas(D))
 paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
     using G = PdGeometry<D>;
     constexpr uint32_t kSteps = D / 16, kR = G::kSlices, kStep = G::kStep;
@@ -867,7 +868,7 @@ static PagedDecodeLayout pd_layout(const tatara_paged_cache& c, uint32_t n_lanes
 template <typename T, int D, int kTiles>
 static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, PagedDecodeParams p) {
     using G = PdGeometry<D>;
-    constexpr uint32_t kCtas = pd_ctas(D, kTiles == 2);
+    constexpr uint32_t kCtas = pd_ctas(D);
     static bool configured[64] = {false};
     if (!configured[ctx->device & 63]) {
         if (cudaFuncSetAttribute(paged_decode_kernel<T, D, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem(G::units(1u), kTiles == 2)) != cudaSuccess)
@@ -880,7 +881,12 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     // Asking ahead pays for long partitions (one lane of 262144 slots 86.5 -> 83.3 us, of 131072 with head_dim 128 49 -> 45), costs 0.2 us
     // where they are the shortest, and slows the arithmetic-bound wide groups (28 -> 32 us).
     p.ahead_slots = items <= kCtas * sms && kTiles == 1 && p.cut.part_slots(p.max_keys) > p.cut.least ? ctx->decode_l2_prefetch_keys : 0u;
-    (void)launch_staged(paged_decode_kernel<T, D, kTiles>, dim3(uint32_t(items < kCtas * sms ? items : kCtas * sms)), kPdThreads, G::smem(p.units, kTiles == 2), stream, p);
+    // Shared memory for just the CTAs that are to share an SM, the rest stays L1 -- and one CTA an SM stays one (one lane of 32768 slots 18.1 ->
+    // 16.9 us against the driver's choice).
+    constexpr uint32_t kSmMemory = 228u * 1024u, kReserved = 1024u;   // of a CTA
+    const uint32_t smem = G::smem(p.units, kTiles == 2), share = (ctas * (smem + kReserved) * 100u + kSmMemory - 1u) / kSmMemory;
+    const dim3 grid(uint32_t(items < kCtas * sms ? items : kCtas * sms));
+    (void)launch_staged_carved(int(share < 100u ? share : 100u), paged_decode_kernel<T, D, kTiles>, grid, kPdThreads, smem, stream, p);
     const tatara_status st = check_launch(ctx, "attn_decode_paged");
     if (st != TATARA_OK) return st;
     const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
