@@ -163,9 +163,9 @@ __device__ __forceinline__ void tc_prepare_units(const uint32_t bar_id, const CU
     // Thread kPrStoreThread hands the four plane images of a unit to the copy engine (thread 0 only the Us^T image,
     // in the middle of the unit) and owns what follows from that, each at a point where it would otherwise idle:
     //  * the images must have LEFT shared memory before the next unit writes over them: it waits for that
-    //    (`wait_group.read`) during the next unit's first MMA group, before the barrier in front of the masks -- the
-    //    next unit's K and Q tiles load into a region that holds no image, and its V tile is asked for after that
-    //    barrier (V is not needed before the second MMA group).  Waiting at the end of the unit held the whole
+    //    (`wait_group.read`) during the next unit's first MMA group, before the barrier in front of the masks (-M', O0^T)
+    //    and the one behind them (Q~^T) -- the next unit's K and Q tiles load into a region that holds no image, and its
+    //    V tile is asked for after those barriers (V is not needed before the second MMA group).  Waiting at the end of the unit held the whole
     //    group for 2.3 - 4.2 k cycles per unit.
     //  * the unit's ready word may only be released once the images are COMPLETE in global memory: it waits for that
     //    (`wait_group 0`) and stores the word (`st.release.gpu`) while warps 0 and 1 invert the diagonal blocks of
@@ -261,7 +261,7 @@ __device__ __forceinline__ void tc_prepare_units(const uint32_t bar_id, const CU
         tc_commit(bar_mma);
     }
     // the previous unit's -M' image (over V, A) and its O0^T image (over P) have left shared memory: the masks write
-    // P and A; the Q~^T image (over T, written by the sweep) may still be on its way
+    // P and A; the Q~^T image (over T) may still be on its way
     if (tid == kPrStoreThread) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
     if (ok) ok = mbar_wait(bar_mma, mma_phase & 1u, abort_flag);
     ++mma_phase;
@@ -294,6 +294,8 @@ __device__ __forceinline__ void tc_prepare_units(const uint32_t bar_id, const CU
         }
         tc_fence_before();
     }
+    // ... and so has its Q~^T image, before anyone writes T over it (an image still on its way left with T's f32 words in it)
+    if (tid == kPrStoreThread) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     group_sync(bar_id);
     if (tid == 0 && ok) {   // V is not needed before the second MMA group
         mbar_expect_tx(bar_v, 16384u);

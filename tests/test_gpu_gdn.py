@@ -484,6 +484,46 @@ def test_chunked_prefill_one_launch_hand_over_on_poisoned_scratch(ctx):
         ctx.set_policy(tb.POLICY_GDN_CHUNK_FORM, 0)
 
 
+def test_chunked_prefill_bits_beside_memory_traffic(ctx):
+    """The preparation hands its plane images to the copy engine and builds the next unit over their shared memory.  With the
+    memory kept busy by copies on another stream the images leave late; the bits are those of a run by itself."""
+    rows = 16384
+    g = torch.Generator(device="cuda").manual_seed(78)
+    x = torch.randn((rows, 32, 128), generator=g, device="cuda")
+    x = x / x.norm(dim=-1, keepdim=True)
+    qk = torch.cat([(x[:, :16] / 128 ** 0.5).reshape(rows, 2048), x[:, 16:].reshape(rows, 2048)], 1).to(torch.bfloat16).contiguous()
+    v = torch.randn((rows, 4096), generator=g, device="cuda").to(torch.bfloat16)
+    decay = torch.exp(-0.5 * torch.rand((rows, 32), generator=g, device="cuda")).contiguous()
+    beta = torch.sigmoid(torch.randn((rows, 32), generator=g, device="cuda")).contiguous()
+    s0 = torch.randn((32, 128, 128), generator=g, device="cuda") * 0.05
+    scratch = chunk_scratch(rows)
+    busy = torch.zeros((2, 1 << 30), dtype=torch.uint8, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    want = None
+    try:
+        for form in (2, 0):
+            ctx.set_policy(tb.POLICY_GDN_CHUNK_FORM, form)
+            for it in range(10):
+                y = torch.zeros((rows, 4096), dtype=torch.bfloat16, device="cuda")
+                s1 = torch.zeros_like(s0)
+                torch.cuda.synchronize()
+                if want is not None:
+                    with torch.cuda.stream(side):
+                        for _ in range(4):
+                            busy[1].copy_(busy[0])
+                ctx.gdn_prefill(qk, v, decay, beta, s0, y, s1, rows, chunk=64, scratch=scratch)
+                torch.cuda.synchronize()
+                ctx.sync()
+                if want is None:
+                    assert torch.isfinite(y.float()).all() and y.float().abs().max() < 1e3 and torch.isfinite(s1).all()
+                    want = (y, s1)
+                else:
+                    assert torch.equal(y, want[0]) and torch.equal(s1, want[1]), f"form {form}, run {it}"
+    finally:
+        ctx.set_policy(tb.POLICY_GDN_CHUNK_FORM, 0)
+
+
 def test_chunked_prefill_config3_full_size(ctx):
     """Benchmark config 3: 16384 rows, chunk 64, initial state zero; per-token outputs and the
     final f32 state against the sequential oracle."""
