@@ -4,7 +4,7 @@
 //
 // One pass over K and V with a running maximum and sum.  A lane's slots are cut into partitions; a work item
 // (lane, kv head, partition) leaves, for every query head of the group, the un-normalised sum of its values, the
-// maximum m of its scores (times log2 e) and the sum l of 2^(s - m).  The join weighs the partitions with 2^(m - M),
+// maximum m of its scores (times log2 e) and the sum l of 2^(s - m) (f16: both sums times 2^14).  The join weighs the partitions with 2^(m - M),
 // divides and applies the gate; where the cache carries a mass it adds 2^(s - M) / L of every slot, summed over the
 // group, to it -- the scores were put aside in f32 by the first kernel, 4 bytes a head beside the 4 x head_dim of K and V.
 //
@@ -57,7 +57,7 @@ struct PagedDecodeParams {
     const uint8_t* gate;
     uint8_t* out;
     float* sums;       // [lane][q head][part][head_dim]
-    float2* stats;     // [lane][q head][part]: maximum (log2 units), sum
+    float2* stats;     // [lane][q head][part]: maximum (log2 units), sum of weights (2^kTopLog2 at the maximum)
     float* scores;     // [lane][kv head][max_keys rounded up to 16][group rounded up to 8], log2 units; null without a mass
     uint64_t query_stride;
     uint32_t n_lanes, max_keys, q_heads, group;
@@ -70,8 +70,12 @@ struct PagedDecodeParams {
     float scale_log2e;
 };
 
+// kTopLog2: the weight of a warp's largest score, in log2 units.  f16 has 2^-14 as its smallest normal number and 2^-24 as its smallest step:
+// with 2^14 for the largest, a weight is normal down to 2^-28 of it and what is lost stays below 2^-39 of it each, 2^-21 over the longest
+// lane, where weights up to 1 would lose 2^-25 each.  Sums and their records all carry the factor, which the quotient takes out again.
 template <typename T> struct Half;
 template <> struct Half<__nv_bfloat16> {
+    static constexpr float kTopLog2 = 0.0f;
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -84,6 +88,7 @@ template <> struct Half<__nv_bfloat16> {
     static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v); }
 };
 template <> struct Half<__half> {
+    static constexpr float kTopLog2 = 14.0f;
     static __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -186,6 +191,14 @@ __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// The weight of a score that lies `below` (not above 0) from the maximum.  The factor goes to the difference, which is 0 at the maximum whatever
+// its size; a large score would round it away.
+template <typename T>
+__device__ __forceinline__ float weight_of(float below) {
+    if constexpr (Half<T>::kTopLog2 != 0.0f) below += Half<T>::kTopLog2;
+    return exp2_fast(below);
 }
 
 // kTiles: tiles of eight query heads, 1 or 2.  Measured with the join, 2 kv heads of 256, 16 query heads, bf16: one lane of 262144 slots 84 us
@@ -521,8 +534,8 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                 const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
 #pragma unroll
                 for (uint32_t i = 0; i < kR; ++i) {
-                    const float p0 = exp2_fast(s[i][nt][0] - b0), p1 = exp2_fast(s[i][nt][1] - b1);
-                    const float p2 = exp2_fast(s[i][nt][2] - b0), p3 = exp2_fast(s[i][nt][3] - b1);
+                    const float p0 = weight_of<T>(s[i][nt][0] - b0), p1 = weight_of<T>(s[i][nt][1] - b1);
+                    const float p2 = weight_of<T>(s[i][nt][2] - b0), p3 = weight_of<T>(s[i][nt][3] - b1);
                     l[nt][0] += p0 + p2;
                     l[nt][1] += p1 + p3;
                     // the weights are rounded to the cache's type for the second product: half a step each, of random sign
@@ -809,7 +822,7 @@ paged_join_kernel(const __grid_constant__ PagedDecodeParams p, const uint32_t wa
             }
 #pragma unroll
             for (uint32_t off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-            if (lane == 0) final_ml[h] = make_float2(top == -INFINITY ? 0.0f : top, sum == 0.0f ? 0.0f : 1.0f / sum);
+            if (lane == 0) final_ml[h] = make_float2(top == -INFINITY ? 0.0f : top, sum == 0.0f ? 0.0f : exp2f(Half<T>::kTopLog2) / sum);
         }
         __syncthreads();
         constexpr uint32_t kOwn = kMassSpan / kJoinThreads;
