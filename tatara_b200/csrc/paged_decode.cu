@@ -84,6 +84,12 @@ template <> struct Half<__nv_bfloat16> {
         const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&v);
     }
+    static __device__ __forceinline__ uint32_t pack_down(float lo, float hi) {
+        uint32_t v;
+        asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+        return v;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
     static __device__ __forceinline__ float load(const uint8_t* p) { return __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(p)); }
     static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v); }
 };
@@ -97,6 +103,12 @@ template <> struct Half<__half> {
         const __half2 v = __floats2half2_rn(lo, hi);
         return *reinterpret_cast<const uint32_t*>(&v);
     }
+    static __device__ __forceinline__ uint32_t pack_down(float lo, float hi) {
+        uint32_t v;
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+        return v;
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
     static __device__ __forceinline__ float load(const uint8_t* p) { return __half2float(*reinterpret_cast<const __half*>(p)); }
     static __device__ __forceinline__ void store(uint8_t* p, float v) { *reinterpret_cast<__half*>(p) = __float2half_rn(v); }
 };
@@ -199,6 +211,17 @@ template <typename T>
 __device__ __forceinline__ float weight_of(float below) {
     if constexpr (Half<T>::kTopLog2 != 0.0f) below += Half<T>::kTopLog2;
     return exp2_fast(below);
+}
+
+// A weight for the second product, as the sum of two numbers of the cache's type: what lies below it and what that leaves, rounded.  One number would
+// be off by half a step (bf16 2^-8, f16 2^-11 of the weight), two are by half a step of the rest: 2^-14.9 and 2^-20.6.  The first is cut from a
+// little less than the weight, so that the rest is above 0 too (f16: down to 2^-27 of the largest weight) and an infinite value stays one.
+template <typename T>
+__device__ __forceinline__ void two_terms(float p0, float p1, uint32_t& most, uint32_t& rest) {
+    constexpr float kLess = 1.0f - 1.0f / 4096.0f;
+    most = Half<T>::pack_down(p0 * kLess, p1 * kLess);
+    const float2 m = Half<T>::unpack(most);
+    rest = Half<T>::pack(p0 - m.x, p1 - m.y);
 }
 
 // kTiles: tiles of eight query heads, 1 or 2.  Measured with the join, 2 kv heads of 256, 16 query heads, bf16: one lane of 262144 slots 84 us
@@ -528,7 +551,7 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                     }
                 }
             }
-            uint32_t pb[kR][kTiles][2];
+            uint32_t pb[kR][kTiles][2], rest[kR][kTiles][2];
 #pragma unroll
             for (uint32_t nt = 0; nt < kTiles; ++nt) {
                 const float b0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], b1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
@@ -538,9 +561,12 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                     const float p2 = weight_of<T>(s[i][nt][2] - b0), p3 = weight_of<T>(s[i][nt][3] - b1);
                     l[nt][0] += p0 + p2;
                     l[nt][1] += p1 + p3;
-                    // the weights are rounded to the cache's type for the second product: half a step each, of random sign
-                    pb[i][nt][0] = movmatrix_trans(Half<T>::pack(p0, p1));   // slots 2t, 2t+1 of head g
-                    pb[i][nt][1] = movmatrix_trans(Half<T>::pack(p2, p3));   // slots 2t+8, 2t+9 of head g
+                    two_terms<T>(p0, p1, pb[i][nt][0], rest[i][nt][0]);
+                    two_terms<T>(p2, p3, pb[i][nt][1], rest[i][nt][1]);
+                    pb[i][nt][0] = movmatrix_trans(pb[i][nt][0]);            // slots 2t, 2t+1 of head g
+                    pb[i][nt][1] = movmatrix_trans(pb[i][nt][1]);            // slots 2t+8, 2t+9 of head g
+                    rest[i][nt][0] = movmatrix_trans(rest[i][nt][0]);
+                    rest[i][nt][1] = movmatrix_trans(rest[i][nt][1]);
                 }
             }
             await_unit();
@@ -552,7 +578,10 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
                     uint32_t a0, a1, a2, a3;
                     ldmatrix_x4_trans(vst + i * kPagedSlice * G::kRow + ks / 4u * 128u + (((ks % 4u * 2u + v_chunk) ^ lm_r) << 4), a0, a1, a2, a3);
 #pragma unroll
-                    for (uint32_t nt = 0; nt < kTiles; ++nt) Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                    for (uint32_t nt = 0; nt < kTiles; ++nt) {
+                        Half<T>::mma(o[nt][ks], a0, a1, a2, a3, rest[i][nt][0], rest[i][nt][1]);
+                        Half<T>::mma(o[nt][ks], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                    }
                 }
             }
             release_unit();

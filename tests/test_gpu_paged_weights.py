@@ -88,3 +88,65 @@ def test_f16_scores_whose_size_leaves_no_room(ctx):
     mean = c.rows(c.values, 0, 0, 50).double().mean(dim=0)
     assert ((out[0].double() - mean).abs() <= 2.0 ** -11 * mean.abs() + 2.0 ** -17 * c.rows(c.values, 0, 0, 50).double().abs().mean(dim=0) + 2.0 ** -25).all()
     assert ((c.mass.double() - before)[0, 0, :50] - 4 / 50).abs().max() <= 2.0 ** -20
+
+
+# A weight is the sum of two numbers of the type: the second is off by half a step of what the first leaves, a step and 2^-12 of the weight at most.
+LOST = {t: u * (2 * u + 2.0 ** -12) for t, u in U.items()}
+LEAST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -39}      # f16: half of its smallest step, for weights up to 2^14
+LAYOUTS = [(2, 8, 256, 16), (1, 16, 256, 48), (8, 4, 128, 16), (2, 11, 128, 64), (12, 1, 64, 32), (2, 16, 64, 16), (3, 5, 64, 112)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kv_heads,group,dim,page", LAYOUTS)
+def test_values_that_cancel(ctx, dtype, kv_heads, group, dim, page):
+    """Slots 2i and 2i + 1 hold nearly the same key and opposite values: what is left of the sum is the difference of two weights."""
+    lens = [2, 40, 130, 1000, 4000]
+    c = Cache(lens, kv_heads, dim, dtype=dtype, page=page, seed=page + dim)
+    for lane, n in enumerate(lens):
+        s = torch.arange(0, n, 2, device="cuda")
+        pair = [(c.table[lane, x // page].long(), slice(None), x % page) for x in (s, s + 1)]
+        c.values[pair[1]] = -c.values[pair[0]]
+        c.keys[pair[1]] = c.keys[pair[0]]
+        c.keys[pair[1] + (5,)] *= 0.9
+    q = (0.2 * torch.randn((len(lens), kv_heads * group, dim), generator=c.gen, device="cuda")).to(dtype)
+    scale = dim ** -0.5
+    want, bound, added, added_bound = definition(c, q, scale, LOST[dtype], LEAST[dtype])
+    before = c.mass.double()
+    out = decode(ctx, c, q, scale)
+    assert ((out.double() - want).abs() <= bound).all()
+    assert ((c.mass.double() - before - added).abs() <= added_bound + 2.0 ** -24 * (before + added)).all()
+
+
+@pytest.mark.parametrize("kv_heads,group,dim,lens", [(2, 8, 256, [100, 700, 17]), (8, 4, 128, [5003]), (1, 1, 64, [262144]), (3, 16, 64, [3000, 33])])
+def test_f16_slots_far_below_lose_hardly_anything(ctx, kv_heads, group, dim, lens):
+    """As above, held to what two numbers of the type lose, the slots at every distance from the one that dominates."""
+    c = Cache(lens, kv_heads, dim, dtype=torch.float16, page=64, seed=dim + group)
+    q = torch.zeros((len(lens), kv_heads * group, dim), dtype=torch.float16, device="cuda")
+    q[:, :, 3] = 1.0
+    spread = 22 * torch.rand(c.keys.shape[:-1], generator=c.gen, device="cuda")
+    c.keys[..., 3] = torch.where(torch.isnan(c.keys[..., 3]), float("nan"), spread).half()
+    for lane, n in enumerate(lens):
+        c.values[int(c.table[lane, (n // 2) // 64]), :, (n // 2) % 64] = 0.0
+        c.keys[int(c.table[lane, (n // 2) // 64]), :, (n // 2) % 64, 3] = 30.0
+    want, bound, _, _ = definition(c, q, 1.0, LOST[torch.float16], LEAST[torch.float16])
+    assert ((decode(ctx, c, q, 1.0).double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("kv_heads,group,dim,page", LAYOUTS)
+def test_infinite_values_stay_infinite(ctx, dtype, kv_heads, group, dim, page):
+    """A value that overflowed makes its dim infinite, with its sign, wherever its slot lies, the largest weight's and a lane's only one included."""
+    lens = [1, 60, 700]
+    c = Cache(lens, kv_heads, dim, dtype=dtype, page=page, seed=page)
+    q = (0.3 * torch.randn((len(lens), kv_heads * group, dim), generator=c.gen, device="cuda")).to(dtype)
+    plain = decode(ctx, c.clone(), q, dim ** -0.5)
+    for lane, n in enumerate(lens):
+        for i, slot in enumerate({0, n // 2, n - 1}):
+            c.values[int(c.table[lane, slot // page]), :, slot % page, 7 * i] = float("inf")
+            c.values[int(c.table[lane, slot // page]), :, slot % page, 7 * i + 1] = -float("inf")
+    out = decode(ctx, c, q, dim ** -0.5)
+    for lane, n in enumerate(lens):
+        dims = [7 * i for i in range(len({0, n // 2, n - 1}))]
+        assert (out[lane][:, dims] == float("inf")).all() and (out[lane][:, [d + 1 for d in dims]] == -float("inf")).all()
+        rest = [d for d in range(dim) if d not in dims and d - 1 not in dims]
+        assert torch.equal(out[lane][:, rest], plain[lane][:, rest])
