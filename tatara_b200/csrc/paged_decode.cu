@@ -654,9 +654,19 @@ paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
             }
             // every warp has read this item's query: the next one's takes its place
             if (nt == 0u) store_query();
-            // half of the descriptors lie behind every warp: the half after the other one takes their place
-            if (nt + 1u == kTiles && done_items % (kPdItems / 2u) == 0u && threadIdx.x < kPdItems / 2u)
-                describe(done_items + kPdItems / 2u + threadIdx.x);
+            // half of the descriptors lie behind every warp's arithmetic: the half after the other one takes their place
+            if (nt + 1u == kTiles && done_items % (kPdItems / 2u) == 0u) {
+                if (threadIdx.x < kPdItems / 2u) describe(done_items + kPdItems / 2u + threadIdx.x);
+                // A warp without a share in a run of items has not read ahead past them and may stand among the replaced: it goes on from the
+                // item under way (left there, it would take descriptors of 128 items on for those it passes).
+                if (at < done_items && done_items < count) {
+                    at = done_items;
+                    turn = 0;
+                    pi = items[at % kPdItems];
+                    settle(pi, 0u, fetch_pages(pi, 0u));
+                    if (at + 1u < count) next_pages = fetch_pages(items[(at + 1u) % kPdItems], 0u);
+                }
+            }
             __syncthreads();
         }
     }
