@@ -537,7 +537,9 @@ tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream, const tata
  * move, in ascending order, into the slots below `keep` that were given up, in ascending order -- K and V rows,
  * mass and position.  So no row moves that need not.  Slots from `keep` on are left as they are; tatara_paged_lanes_step
  * then cuts the lane.  Needs mass, and positions where recent > 0; sink + recent <= keep.  Pages that two lanes share may
- * hold only their first `sink` slots (nothing there is ever overwritten). */
+ * hold only their first `sink` slots (nothing there is ever overwritten).  With keep >= max_keys no lane can have anything to
+ * trim: the call enqueues nothing and looks at no lane, so it is the one call that does not report a lane with more than
+ * max_keys slots.  A caller that then cuts with tatara_paged_lanes_step gives max_keys as large as any lane may have become. */
 uint64_t tatara_paged_evict_scratch_bytes(const tatara_paged_cache* cache, uint32_t n_lanes, uint32_t max_keys,
                                           uint32_t keep);
 tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,

@@ -498,7 +498,8 @@ class Context:
             out.data_ptr(), scratch_at, scratch_bytes))
 
     def paged_evict(self, cache, lanes, keep, scratch, sink=0, recent=0, max_keys=None, stream=None):
-        """Trims every lane to at most `keep` slots; paged_lanes_step(lanes, keep=keep) then cuts the lane table."""
+        """Trims every lane to at most `keep` slots; paged_lanes_step(lanes, keep=keep) then cuts the lane table.  keep >= max_keys: nothing is
+        done, and no lane is looked at."""
         at, n = self._paged_lanes(lanes, cache)
         scratch_at, scratch_bytes = self._paged_scratch(scratch, cache)
         self._check(lib().tatara_paged_evict(

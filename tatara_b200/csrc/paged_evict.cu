@@ -497,7 +497,7 @@ extern "C" tatara_status tatara_paged_evict(tatara_ctx* ctx, void* stream, const
     const uint64_t rows = uint64_t(n_lanes) * cache->kv_heads;
     const PagedEvictLayout layout = evict_layout(rows, max_keys, keep);
     if (scratch_bytes < layout.bytes) return fail(ctx, TATARA_SCRATCH_TOO_SMALL, "paged_evict: scratch");
-    if (layout.room == 0u) return TATARA_OK;   // no lane can hold more than keep
+    if (layout.room == 0u) return TATARA_OK;   // no lane of max_keys slots holds more than keep; none is looked at
     PagedEvictParams p{};
     p.cache = paged_view(ctx, *cache);
     p.lanes = lanes_device;
