@@ -511,7 +511,9 @@ tatara_status tatara_paged_append(tatara_ctx* ctx, void* stream, const tatara_pa
 /* tatara_attn_qk_rope_batch over pages: projection row i [9216] belongs to lane i; q / gate rows as there, K and V
  * to slot keys - 1 at the lane's position.  bf16, 2 kv heads of 256.  The angle is reduced in double and each
  * result rounded once, so rows agree with tatara_attn_qk_rope_batch (which rounds the normalised row to
- * bf16 first) within that operator's roundings.  Idle lanes' q and gate rows stay as they are. */
+ * bf16 first) within that operator's roundings: two half steps of the normalised row, and its angle, position / divisor in
+ * f32, half a step of which is 2^-24 of the angle -- 2^-7 rad at the longest context.  A lane whose prompt was rotated there
+ * and whose tokens are rotated here holds keys of both.  Idle lanes' q and gate rows stay as they are. */
 tatara_status tatara_attn_qk_rope_paged(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
                                         const tatara_paged_lane* lanes_device, uint32_t n_lanes,
                                         const void* projection, const void* q_weight, const void* k_weight,
