@@ -944,12 +944,15 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     const uint32_t pieces = p.n_lanes * p.q_heads * (D / kJoinDims);
     const uint64_t spans = uint64_t(p.n_lanes) * p.cache.kv_heads * ((p.max_keys + kMassSpan - 1u) / kMassSpan);
     const uint32_t walkers = p.cache.mass == nullptr ? 0u : uint32_t(spans < 4u * ctx->sm_count ? spans : 4u * ctx->sm_count);
-    if (p.parts <= 16u)
-        (void)launch_staged(paged_join_kernel<T, D, kJoinWarp>, dim3((pieces + kJoinWarps - 1u) / kJoinWarps + walkers), kJoinThreads, 0u, stream, p, walkers);
-    else if (D != 64 && pieces > 4u * sms)
-        (void)launch_staged(paged_join_kernel<T, D, kJoinHead>, dim3(p.n_lanes * p.q_heads + walkers), kJoinThreads, 0u, stream, p, walkers);
-    else
-        (void)launch_staged(paged_join_kernel<T, D, kJoinSlice>, dim3(pieces + walkers), kJoinThreads, 0u, stream, p, walkers);
+    auto join = p.parts <= 16u ? paged_join_kernel<T, D, kJoinWarp> : paged_join_kernel<T, D, kJoinSlice>;
+    uint32_t join_ctas = p.parts <= 16u ? (pieces + kJoinWarps - 1u) / kJoinWarps : pieces;
+    if constexpr (D != kJoinDims) {   // (a slice is a head there)
+        if (p.parts > 16u && pieces > 4u * sms) {
+            join = paged_join_kernel<T, D, kJoinHead>;
+            join_ctas = p.n_lanes * p.q_heads;
+        }
+    }
+    (void)launch_staged(join, dim3(join_ctas + walkers), kJoinThreads, 0u, stream, p, walkers);
     return check_launch(ctx, "attn_decode_paged: join");
 }
 
