@@ -35,8 +35,7 @@ struct PagedEvictParams {
     uint32_t move_blocks, warp_pairs;   // blocks of the second kernel for each row, pairs of a warp (at most 32)
 };
 
-struct SelectShared {
-    uint32_t hist[3][kSelBins];
+struct SelectShared {                // beside the histograms
     uint4 warp_counts[kSelWarps];
     uint32_t warp_sum[kSelWarps];
     uint32_t bin, above;             // the digit that holds the threshold, keys beyond it
@@ -233,9 +232,10 @@ __device__ __forceinline__ void write_lists(const PagedEvictParams& p, uint32_t 
 template <uint32_t kKeys>
 __global__ void __launch_bounds__(kSelThreads, 1)
 paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
-    __shared__ __align__(16) SelectShared sh;
+    __shared__ SelectShared sh;
+    __shared__ __align__(8) uint32_t hist[3][kSelBins];
     const uint32_t row = blockIdx.x, lane_row = row / p.cache.kv_heads, head = row - lane_row * p.cache.kv_heads;
-    for (uint32_t i = threadIdx.x; i < 3u * kSelBins; i += kSelThreads) (&sh.hist[0][0])[i] = 0u;
+    for (uint32_t i = threadIdx.x; i < 3u * kSelBins; i += kSelThreads) (&hist[0][0])[i] = 0u;
     wait_for_predecessor();
     release_dependents();
     const uint2 l = __ldcg(reinterpret_cast<const uint2*>(p.lanes + lane_row));   // keys, position
@@ -254,9 +254,9 @@ paged_select_kernel(const __grid_constant__ PagedEvictParams p) {
     uint32_t prefix = 0u, want = p.keep;
 #pragma unroll
     for (uint32_t digit = 0; digit < 3u; ++digit) {
-        add_digit(sh.hist[digit], s, digit, prefix);
+        add_digit(hist[digit], s, digit, prefix);
         __syncthreads();
-        find_digit(sh.hist[digit], false, digit, sh, prefix, want);
+        find_digit(hist[digit], false, digit, sh, prefix, want);
     }
     uint4 all;
     const uint4 c = count_slots(p, s, prefix), b = counts_before(sh, c, all);
@@ -341,8 +341,9 @@ paged_search_keys_kernel(const __grid_constant__ PagedEvictParams p) {
 template <uint32_t kKeys>
 __global__ void __launch_bounds__(kSelThreads, 1)
 paged_search_digit_kernel(const __grid_constant__ PagedEvictParams p, const uint32_t digit) {
-    __shared__ __align__(16) SelectShared sh;
-    clear_hist(sh.hist[0]);
+    __shared__ SelectShared sh;
+    __shared__ uint32_t next[kSelBins];
+    clear_hist(next);
     wait_for_predecessor();
     release_dependents();
     SlotKeys<kKeys> s;
@@ -355,8 +356,8 @@ paged_search_digit_kernel(const __grid_constant__ PagedEvictParams p, const uint
     find_digit(hist, true, digit, sh, so_far.x, so_far.y);
     if (w.block == 0u && threadIdx.x == 0u) p.found[w.row * 4u + digit + 1u] = so_far;
     if (digit != 2u) {
-        add_digit(sh.hist[0], s, digit + 1u, so_far.x);
-        add_up(hist + kSelBins, sh.hist[0]);
+        add_digit(next, s, digit + 1u, so_far.x);
+        add_up(hist + kSelBins, next);
     } else {
         uint4 all;
         (void)counts_before(sh, count_slots(p, s, so_far.x), all);
@@ -367,7 +368,7 @@ paged_search_digit_kernel(const __grid_constant__ PagedEvictParams p, const uint
 template <uint32_t kKeys>
 __global__ void __launch_bounds__(kSelThreads, 1)
 paged_search_lists_kernel(const __grid_constant__ PagedEvictParams p) {
-    __shared__ __align__(16) SelectShared sh;
+    __shared__ SelectShared sh;
     wait_for_predecessor();
     release_dependents();
     SlotKeys<kKeys> s;
