@@ -502,7 +502,8 @@ typedef struct tatara_paged_cache {
  * [n_lanes + 1], ascending from 0; rows from row_starts[n_lanes] up to n_rows (padding) are not read.
  * row_starts == NULL: row i belongs to lane i (n_rows == n_lanes).  The slots' mass is set to 0 and their
  * positions to the tokens'.  A row whose slot would lie before slot 0 or beyond the page table is left out, and so
- * are rows that row_starts counts beyond n_rows; either latches TATARA_CONTEXT_OUT_OF_RANGE. */
+ * are rows that row_starts counts beyond n_rows; either latches TATARA_CONTEXT_OUT_OF_RANGE.  Rows of an idle lane are
+ * left out without a report. */
 tatara_status tatara_paged_append(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,
                                   const tatara_paged_lane* lanes_device, uint32_t n_lanes, const void* keys,
                                   const void* values, uint64_t row_stride, uint64_t source_head_stride,
@@ -525,7 +526,9 @@ tatara_status tatara_attn_qk_rope_paged(tatara_ctx* ctx, void* stream, const tat
  * at most TATARA_MAX_GROUP per kv head; softmax(scale * q.k) v, times sigmoid(gate).  With cache->mass every slot's
  * weight, summed over the query heads of its kv head, is added to its mass.  An idle lane's out row becomes
  * zero.  max_keys: no lane holds more slots (it bounds the scratch; the
- * page table's capacity serves when nothing better is known).  A lane's bits do not depend on the batch. */
+ * page table's capacity serves when nothing better is known); TATARA_MAX_CONTEXT at most, the scratch size is 0 beyond it.
+ * Scores, sums and the mass are f32; a weight enters the product with V as two numbers of the cache's type, off by
+ * 2^-14.9 (bf16) or 2^-20.6 (f16) of itself.  A lane's bits do not depend on the batch. */
 uint64_t tatara_attn_decode_paged_scratch_bytes(const tatara_paged_cache* cache, uint32_t n_lanes, uint32_t max_keys,
                                                 uint32_t q_heads);
 tatara_status tatara_attn_decode_paged(tatara_ctx* ctx, void* stream, const tatara_paged_cache* cache,

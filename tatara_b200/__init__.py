@@ -484,7 +484,7 @@ class Context:
 
     def attn_decode_paged(self, cache, lanes, q, gate, out, scratch, max_keys=None, scale=None, stream=None):
         """q, gate (or None), out: [lane][q head][dim], rows of any one stride.  Adds to the cache's mass where it has one.
-        scale: head_dim ** -0.5 unless given; max_keys: the page table's capacity unless given."""
+        scale: head_dim ** -0.5 unless given; max_keys: the page table's capacity, MAX_CONTEXT at most, unless given."""
         at, n = self._paged_lanes(lanes, cache)
         q_heads, dim = q.shape[1], cache.head_dim
         stride = self._paged_rows("attn_decode_paged: q", q, cache, n, q_heads * dim)

@@ -100,7 +100,7 @@ paged_append_kernel(const __grid_constant__ PagedAppendParams p) {
 // A warp owns one (head, row): lane l holds dims 8l .. 8l+7 (16-byte accesses), dims d and d + 32 of a rotated pair are
 // four lanes apart.  Lane l evaluates the angle of pair l, in turns: the product and the fraction in double, since a far position
 // loses its angle in f32 (2^18 / 1.6 has a last place of 1/64), then one sincospif; lanes 0 .. 7 take theirs by shuffles.  Latency
-// bound: 2.4 us for 8 lanes, 4.0 for 256 (9.4 MB).
+// bound: 2.4 us for 8 lanes, 4.4 for 256 (9.4 MB).
 constexpr uint32_t kRopeWarps = 4;
 
 // Turns of each pair from one position to the next; the model's divisors are base^(pair / 32) rounded to f32.

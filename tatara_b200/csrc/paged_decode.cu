@@ -214,7 +214,9 @@ __device__ __forceinline__ float weight_of(float below) {
 }
 
 // A weight for the second product, as the sum of two numbers of the cache's type: what lies below it and what that leaves, rounded.  One number would
-// be off by half a step (bf16 2^-8, f16 2^-11 of the weight), two are by half a step of the rest: 2^-14.9 and 2^-20.6.  The first is cut from a
+// be off by half a step (bf16 2^-8, f16 2^-11 of the weight), two are by half a step of the rest: 2^-14.9 and 2^-20.6.  The second product's
+// matrix instructions double: 84.0 -> 84.5 us for one lane of 262144 slots, 29.7 -> 30.4 for 96 short lanes of head_dim 64, 57.5 -> 59.0 for 16 lanes
+// of 8192 with 16 query heads a kv head of 256.  The first is cut from a
 // little less than the weight, so that the rest is above 0 too (f16: down to 2^-27 of the largest weight) and an infinite value stays one.
 template <typename T>
 __device__ __forceinline__ void two_terms(float p0, float p1, uint32_t& most, uint32_t& rest) {
@@ -225,8 +227,10 @@ __device__ __forceinline__ void two_terms(float p0, float p1, uint32_t& most, ui
 }
 
 // kTiles: tiles of eight query heads, 1 or 2.  Measured with the join, 2 kv heads of 256, 16 query heads, bf16: one lane of 262144 slots 84 us
-// (6.3 TB/s of K and V, bound by HBM), of 4096 9.3 us (latency), 32 lanes of 16384 185 us (5.8 TB/s); 16 lanes of 8192, 8 kv heads of
-// 128 91 us (5.9 TB/s), of 64 51 us (5.2 TB/s, bound by the instructions of a step).
+// (6.4 TB/s of K and V, bound by HBM), of 4096 8.9 us (latency), 32 lanes of 16384 185 us (5.8 TB/s); 16 lanes of 8192, 8 kv heads of
+// 128 91 us (5.9 TB/s), of 64 52 us (5.2 TB/s, bound by the instructions of a step).  Short lanes of head_dim 64 are bound by what a
+// partition costs beside its one step of each warp -- the join of the warps, its barriers, the record, the next query: 96 lanes of 40 to 1500,
+// 12 kv heads, 30 us (4.0 TB/s).
 template <typename T, int D, int kTiles>
 __global__ void __launch_bounds__(kPdThreads, pd_ctas(D))
 paged_decode_kernel(const __grid_constant__ PagedDecodeParams p) {
@@ -930,11 +934,11 @@ static tatara_status launch_paged_decode(tatara_ctx* ctx, cudaStream_t stream, P
     const uint64_t items = uint64_t(p.n_lanes) * p.parts * p.cache.kv_heads, sms = ctx->sm_count;
     const uint32_t ctas = items >= kCtas * sms ? kCtas : uint32_t((items + sms - 1u) / sms);   // on an SM
     p.units = G::units(ctas);
-    // Asking ahead pays for long partitions (one lane of 262144 slots 86.5 -> 83.3 us, of 131072 with head_dim 128 49 -> 45), costs 0.2 us
+    // Asking ahead pays for long partitions (one lane of 262144 slots 86.7 -> 84.2 us, of 131072 with head_dim 128 48 -> 45), costs 0.2 us
     // where they are the shortest, and slows the arithmetic-bound wide groups (28 -> 32 us).
     p.ahead_slots = items <= kCtas * sms && kTiles == 1 && p.cut.part_slots(p.max_keys) > p.cut.least ? ctx->decode_l2_prefetch_keys : 0u;
-    // Shared memory for just the CTAs that are to share an SM, the rest stays L1 -- and one CTA an SM stays one (one lane of 32768 slots 18.1 ->
-    // 16.9 us against the driver's choice).
+    // Shared memory for just the CTAs that are to share an SM, the rest stays L1 -- and one CTA an SM stays one (one lane of 131072 slots 46.8 ->
+    // 45.4 us against the driver's choice, of 32768 18.8 -> 18.2).
     constexpr uint32_t kSmMemory = 228u * 1024u, kReserved = 1024u;   // of a CTA
     const uint32_t smem = G::smem(p.units, kTiles == 2), share = (ctas * (smem + kReserved) * 100u + kSmMemory - 1u) / kSmMemory;
     const dim3 grid(uint32_t(items < kCtas * sms ? items : kCtas * sms));
